@@ -12,7 +12,8 @@ src/cuda_/build.py:256). Every call goes to libdk_decode.so (HIP, gfx950); there
 PyTorch or CPU fallback, and a missing library raises ImportError.
 
 Differences from the reference, all extensions: bf16 as well as fp16; an fp8 (E4M3) cache
-under fp16/bf16 queries, with per-tensor k_scale / v_scale; any split_kv >= 1
+under fp16/bf16 queries, with per-tensor k_scale / v_scale, and a 4-bit (MXFP4) one with scales of
+its own; any split_kv >= 1
 (the reference allows 1..32), and split_kv=0 or None selects the balanced mode, in which
 a persistent grid gives every wavefront an equal share of all (sequence, kv head, page)
 work whatever the sequence lengths; work runs on torch's current stream of q's device
@@ -31,12 +32,14 @@ from typing import Optional
 import torch
 
 import dk_lib
+import layout
 from dk_lib import DecodeArgumentError
 
 PAGE_SIZE = 16
 SUPPORTED_HEAD_DIMS = (64, 128, 256)
 _DTYPE_CODE = {torch.float16: dk_lib.DK_F16, torch.bfloat16: dk_lib.DK_BF16}
 KV_FP8 = torch.float8_e4m3fn            # OCP E4M3: the fp8 cache format the kernel reads
+KV_FP4 = "mxfp4"                        # what _kv_layout calls a 4-bit cache's element type
 
 
 def _fail(msg: str) -> None:
@@ -47,7 +50,16 @@ def _kv_layout(kv_data):
     """The paged cache in either FlashInfer NHD form: one tensor
     (num_pages, 2, page_size, num_kv_heads, head_dim) with K at [:, 0] and V at [:, 1]
     (src/layout.md:41-69), or a (k_cache, v_cache) pair of (num_pages, page_size,
-    num_kv_heads, head_dim) tensors with equal strides (SGLang's token pools)."""
+    num_kv_heads, head_dim) tensors with equal strides (SGLang's token pools); or a 4-bit
+    cache (layout.alloc_kv4_cache)."""
+    if layout.is_kv4(kv_data):
+        try:
+            d = layout.kv4_head_dim(kv_data)
+        except layout.LayoutError as exc:
+            raise DecodeArgumentError(str(exc)) from None
+        return SimpleNamespace(k=kv_data, v=None, num_pages=kv_data.shape[0], page_size=PAGE_SIZE,
+                               hkv=kv_data.shape[1], d=d, dtype=KV_FP4, device=kv_data.device,
+                               strides=(kv_data.stride(0), 0, 0, kv_data.stride(1)), d_stride=1)
     if isinstance(kv_data, (tuple, list)):
         if len(kv_data) != 2 or not all(isinstance(t, torch.Tensor) for t in kv_data):
             raise TypeError("kv_data must be a tensor or a (k_cache, v_cache) pair of tensors")
@@ -97,14 +109,14 @@ def _check(q, kv_data, kv_indptr, kv_indices, kv_last_page_len, wide_pages=False
         _fail(f"q must be fp16 or bf16, got {q.dtype}")
     if q.dim() != 3:
         _fail(f"q must be 3-D (batch, num_q_heads, head_dim), got shape {tuple(q.shape)}")
-    if kv.dtype != q.dtype and kv.dtype != KV_FP8:
+    if kv.dtype not in (q.dtype, KV_FP8, KV_FP4):
         _fail(f"kv_data dtype {kv.dtype} must match q dtype {q.dtype} (or be "
               f"torch.float8_e4m3fn)")
     if q.shape[2] != kv.d:
         _fail(f"head_dim mismatch: q has {q.shape[2]}, kv_data has {kv.d}")
     if q.shape[2] not in SUPPORTED_HEAD_DIMS:
         _fail(f"head_dim must be 64, 128, or 256; got {q.shape[2]}")
-    if q.shape[1] % kv.hkv != 0:
+    if kv.hkv == 0 or q.shape[1] % kv.hkv != 0:
         _fail(f"num_q_heads ({q.shape[1]}) must be divisible by num_kv_heads ({kv.hkv})")
     for name, t in (("kv_indptr", kv_indptr), ("kv_indices", kv_indices),
                     ("kv_last_page_len", kv_last_page_len)):
@@ -145,11 +157,11 @@ def _contig1d(t: torch.Tensor) -> torch.Tensor:
 
 def _kv_options(kv, k_scale, v_scale):
     """(kv_dtype, k_scale, v_scale) for dk_options: an fp8 cache takes positive finite
-    per-tensor scales (default 1); a cache of q's type takes none."""
+    per-tensor scales (default 1); a cache of q's type or of 4 bits takes none."""
     if kv.dtype != KV_FP8:
         if k_scale not in (None, 1.0) or v_scale not in (None, 1.0):
             _fail("k_scale / v_scale apply to a torch.float8_e4m3fn cache only")
-        return dk_lib.DK_KV_SAME, 0.0, 0.0
+        return dk_lib.DK_KV_MXFP4 if kv.dtype == KV_FP4 else dk_lib.DK_KV_SAME, 0.0, 0.0
     scales = []
     for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
         x = 1.0 if x is None else float(x)
@@ -460,7 +472,8 @@ def decode_attention(
         kv_data          : (num_pages, 2, 16, num_kv_heads, head_dim), q's dtype or
                            torch.float8_e4m3fn (NHD), or a (k_cache, v_cache) pair of
                            (num_pages, 16, num_kv_heads, head_dim) tensors with equal
-                           strides
+                           strides, or a 4-bit (OCP MXFP4) cache: uint8 (num_pages,
+                           num_kv_heads, 17 * head_dim), see layout.alloc_kv4_cache
         kv_indptr        : (batch + 1,) int32 CSR row pointer into kv_indices
         kv_indices       : (kv_indptr[-1],) int32 physical page ids
         kv_last_page_len : (batch,) int32 valid tokens in each sequence's last page
@@ -709,6 +722,8 @@ def decode_partials(q, kv_data, kv_indptr, kv_indices, kv_last_page_len, split_k
     kv = _check(q, kv_data, kv_indptr, kv_indices, kv_last_page_len)
     if kv.v is not None:
         _fail("decode_partials takes the combined (num_pages, 2, 16, Hkv, D) cache")
+    if kv.dtype == KV_FP4:
+        _fail("decode_partials does not take a 4-bit cache")
     kv_dtype, k_sc, v_sc = _kv_options(kv, k_scale, v_scale)
     lib = dk_lib.load()
     split = choose_split(q, kv_data, kv_indices) if split_kv in (None, 0) else \

@@ -13,6 +13,7 @@
 
 #include "dk_args.h"
 #include "dk_decode.h"
+#include "dk_kv4.h"
 #include "dk_launch.h"
 
 namespace dk {
@@ -392,6 +393,156 @@ bool short_split_runs(const Problem& p, const Plan& pl, int cus) {
   return groups != cus || pps <= kShortSplitPages;
 }
 
+// ---- the 4-bit cache
+// Explicit split that split_kv == 0 runs (1: one pass), or 0 for the balanced schedule.
+int kv4_auto_split(const Problem& p, const Plan& pl, int cus) {
+  const int64_t pairs = (int64_t)p.batch * pl.pairs_per_seq;
+  const int64_t groups = (int64_t)cus * kKv4WavesPerCU / kKv4Waves;
+  const int64_t hint = p.opt.max_pages_per_seq;
+  int64_t s = 0;
+  if (p.opt.window > 0) {
+    const int64_t avg = p.num_indices / p.batch;
+    const int64_t pages = std::min<int64_t>(avg, p.opt.window / kPageSize + 2);
+    s = std::min(groups / pairs, pages / (2 * kKv4StepPages));
+    s = std::min<int64_t>(std::max<int64_t>(s, 1), kMaxSplit);
+  } else if (p.opt.schedule == 2) {
+    s = 1;
+  } else if (p.opt.schedule == 0 && hint > 0) {
+    const int64_t per = std::max<int64_t>(groups / pl.pairs_per_seq, 1);
+    if (pairs <= groups && hint <= (p.num_indices + per - 1) / per) s = 1;
+  }
+  for (; s > 1; --s) {
+    size_t o, m, l, total;
+    partials_layout_rows(split_rows(p.batch, p.hq, (int)s), p.head_dim, &o, &m, &l, &total);
+    if (total <= p.workspace_bytes) break;
+  }
+  return (int)s;
+}
+
+// Ranges (workgroups per head chunk) of the balanced schedule: about kKv4WavesPerCU wavefronts per
+// CU, no more than leave a wavefront a step of pages each, at most kMaxWaves in all.
+int kv4_ranges(const Problem& p, const Plan& pl, int cus) {
+  const int64_t hc = pl.pairs_per_seq;
+  const int64_t wpc = p.opt.waves_per_cu ? p.opt.waves_per_cu : kKv4WavesPerCU;
+  int64_t r = (std::max<int64_t>((int64_t)cus * wpc / kKv4Waves, 1) + hc / 2) / hc;
+  const int64_t hint = p.opt.max_pages_per_seq;
+  const int64_t pages = hint > 0 ? std::min(p.num_indices, hint * p.batch) : p.num_indices;
+  r = std::min(r, (pages + kKv4StepPages - 1) / kKv4StepPages);
+  return (int)std::max<int64_t>(std::min<int64_t>(r, kMaxWaves / hc), 1);
+}
+
+int run_kv4(Problem p, void* stream) {
+  const int cus = cu_count(current_device(-1));
+  if (cus <= 0) return hip_fail(hipErrorNoDevice, "compute-unit count");
+  Plan pl = make_plan(p);
+  int ranges = 0, seg_cost = 0;
+  if (p.split == 0) {
+    if (const int s = kv4_auto_split(p, pl, cus)) {
+      p.split = s;
+      pl = make_plan(p);
+    } else {
+      ranges = kv4_ranges(p, pl, cus);
+      const int64_t hint = p.opt.max_pages_per_seq;
+      if (hint > 0 && p.batch > 1 && hint * (int64_t)p.batch * 4 > p.num_indices * (int64_t)5)
+        seg_cost = kSegmentCostPerWave * kKv4Waves;
+    }
+  }
+  Pass1Args a{};
+  a.q = static_cast<const uint8_t*>(p.q);
+  a.kv = static_cast<const uint8_t*>(p.kv);
+  a.indptr = p.indptr;
+  a.indices = p.indices;
+  a.last_len = p.last_len;
+  a.out = static_cast<uint8_t*>(p.out);
+  if (p.split != 1) {
+    size_t off_o, off_m, off_l, total;
+    partials_layout_rows(pl.balanced ? balanced_rows(p.batch, p.hq, p.hkv, p.head_dim)
+                                     : split_rows(p.batch, p.hq, p.split),
+                         p.head_dim, &off_o, &off_m, &off_l, &total);
+    if (!p.workspace || total > p.workspace_bytes)
+      return set_error(DK_EWORKSPACE, "internal: partials not assigned for this schedule");
+    uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+    a.part_o = reinterpret_cast<float*>(ws + off_o);
+    a.part_m = reinterpret_cast<float*>(ws + off_m);
+    a.part_l = reinterpret_cast<float*>(ws + off_l);
+  }
+  a.q_b = p.st.q_b * 2;
+  a.q_h = p.st.q_h * 2;
+  a.kv_p = p.st.kv_p;
+  a.kv_h = (int32_t)p.st.kv_h;
+  a.o_b = p.st.o_b * 2;
+  a.o_h = p.st.o_h * 2;
+  a.batch = p.batch;
+  a.hq = p.hq;
+  a.hkv = p.hkv;
+  a.group = pl.group;
+  a.chunks = pl.chunks;
+  a.per = pl.per;
+  a.window = p.opt.window;
+  a.split = std::max(p.split, 1);
+  a.num_indices = (int32_t)p.num_indices;
+  a.num_pages = (uint32_t)std::min<int64_t>(p.num_pages, (int64_t)1 << 31);
+  a.direct = p.split == 1;
+  a.ranges = ranges;
+  a.seg_cost = seg_cost;
+  const float scale = p.opt.sm_scale != 0.f ? p.opt.sm_scale : 1.f / sqrtf((float)p.head_dim);
+  const bool cap = p.opt.logit_cap > 0.f;
+  a.kscale = kLog2e * scale;
+  a.cap_in = cap ? scale / p.opt.logit_cap : 0.f;
+  a.cap_out = cap ? kLog2e * p.opt.logit_cap : 0.f;
+  a.sinks = p.opt.sinks;
+  const int hp = pl.heads <= 4 ? 4 : pl.heads;
+  const bool bf16 = p.dtype == DK_BF16;
+  const void* fn = p.head_dim == 64    ? kv4_symbol<64>(bf16, hp, cap, kKv4Waves, pl.balanced)
+                   : p.head_dim == 128 ? kv4_symbol<128>(bf16, hp, cap, kKv4Waves, pl.balanced)
+                                       : kv4_symbol<256>(bf16, hp, cap, kKv4Waves, pl.balanced);
+  if (!fn) return hip_fail(hipErrorInvalidDeviceFunction, "4-bit decode kernel");
+  int64_t grid = pl.grid;
+  if (pl.balanced) {
+    const int64_t units = (int64_t)p.hkv * ranges;
+    grid = pl.chunks == 1 ? units : (units + kXcds - 1) / kXcds * kXcds * pl.chunks;
+  }
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  {
+    TraceRange tr("dk_kv4 %s B=%d Hq=%d Hkv=%d D=%d split=%d grid=%d",
+                  pl.balanced ? "balanced" : "split", p.batch, p.hq, p.hkv, p.head_dim, p.split,
+                  (int)grid);
+    int heads = pl.heads;
+    void* args[] = {&a, &heads};
+    e = hipLaunchKernel(fn, dim3((uint32_t)grid), dim3(kKv4Waves * 64), args, 0, st);
+  }
+  if (e != hipSuccess) return hip_fail(e, "4-bit decode launch");
+  if (p.split == 1) return DK_OK;
+  MergeArgs m{};
+  m.po = a.part_o;
+  m.pm = a.part_m;
+  m.pl = a.part_l;
+  m.out = a.out;
+  m.o_b = a.o_b;
+  m.o_h = a.o_h;
+  m.batch = p.batch;
+  m.hq = p.hq;
+  m.split = a.split;
+  m.indptr = p.indptr;
+  m.num_indices = a.num_indices;
+  m.pairs_per_seq = pl.pairs_per_seq;
+  m.heads = pl.heads;
+  m.group = pl.group;
+  m.per = pl.per;
+  m.chunks = pl.chunks;
+  m.hkv = p.hkv;
+  m.waves_per_pair = ranges;
+  m.seg_cost = a.seg_cost;
+  m.keep_nan = 1;
+  m.sinks = a.sinks;
+  TraceRange tr("dk_merge %s B=%d Hq=%d D=%d", pl.balanced ? "balanced" : "split", p.batch, p.hq,
+                p.head_dim);
+  e = bf16 ? launch_merge<BF16>(m, p.head_dim, pl.balanced, st)
+           : launch_merge<F16>(m, p.head_dim, pl.balanced, st);
+  return e == hipSuccess ? DK_OK : hip_fail(e, "merge launch");
+}
+
 }  // namespace
 
 // Validation, planning and both passes; shared by the extern "C" entry points.
@@ -399,6 +550,7 @@ int run(Problem p, bool do_merge, void* stream) {
   clear_error();
   const int rc = validate(p);
   if (rc != DK_OK || p.batch == 0) return rc;
+  if (p.kv4()) return run_kv4(p, stream);
   Plan pl = make_plan(p);
   if (!pl.balanced) {
     const int cus = cu_count(current_device(-1));
@@ -721,6 +873,11 @@ int dk_plan_schedule(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, i
   const int dev = dk::current_device(device);
   const int cus = dk::cu_count(dev);
   if (cus <= 0) return dk::hip_fail(hipErrorNoDevice, "dk_plan_schedule");
+  if (p.kv4()) {
+    if (batch == 0) return 0;
+    p.workspace_bytes = dk::workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, 0);
+    return dk::kv4_auto_split(p, dk::make_plan(p), cus);
+  }
   if (p.opt.window > 0)   // explicit splits of the window, in the default workspace
     return dk::window_split(p, cus, dk::workspace_bytes(batch, num_q_heads, num_kv_heads,
                                                         head_dim, 0));

@@ -83,6 +83,16 @@ bool pool_ok(int64_t num_pages, const dk_strides& s, int64_t kv_r, int32_t hkv, 
   return last * esize < ((__int128)1 << 62);
 }
 
+bool kv4_pool_ok(const void* cache, int64_t num_pages, int64_t kv_p, int32_t hkv, int64_t kv_h,
+                 int32_t head_dim) {
+  if (kv_p < 0 || kv_h < 0 || kv_p >= kMaxStride || kv_h >= kMaxStride || kv_p % 16 || kv_h % 16 ||
+      (uintptr_t)cache % 16)
+    return false;
+  const __int128 heads = (__int128)(hkv - 1) * kv_h + 17 * head_dim;
+  return heads < ((__int128)1 << 31) &&
+         ((__int128)std::max<int64_t>(num_pages, 1) - 1) * kv_p + heads < ((__int128)1 << 62);
+}
+
 void partials_layout_rows(int64_t rows, int32_t head_dim, size_t* off_o, size_t* off_m,
                           size_t* off_l, size_t* total) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -143,8 +153,8 @@ Plan make_plan(const Problem& p) {
   // q.k on the VALU by default: its full-row K loads stream faster than the MFMA path's
   // 64-byte row segments on the NHD layout (measured for both fp16 and bf16); groups too
   // large for one VALU chunk take the MFMA path, which holds 16 heads per wavefront
-  pl.mfma = qk_on_mfma(p.opt.qk_path, p.hq / p.hkv, p.head_dim,
-                       p.opt.kv_dtype == DK_KV_FP8_E4M3);
+  pl.mfma = p.kv4() || qk_on_mfma(p.opt.qk_path, p.hq / p.hkv, p.head_dim,
+                                  p.opt.kv_dtype == DK_KV_FP8_E4M3);
   const HeadChunks hc = head_chunks(pl.group, p.head_dim, pl.mfma);
   pl.heads = hc.heads;
   pl.per = hc.per;
@@ -155,6 +165,7 @@ Plan make_plan(const Problem& p) {
                                    : (p.narrow_rows() || (pl.heads >= 8 && !pl.mfma)
                                           ? kDefaultWavesPerGroupNarrow
                                           : kDefaultWavesPerGroup);
+  if (p.kv4()) pl.waves = kKv4Waves;
   pl.kv8 = kv8;
   pl.balanced = p.split == 0;
   pl.grid = pl.balanced ? 0 : split_grid(p.batch, p.hkv, std::max(p.split, 1), pl.chunks);
@@ -204,14 +215,20 @@ int validate(const Problem& p) {
     return set_error(DK_EINVAL,
                      "options.sm_scale must be finite and >= 0 (0 = 1/sqrt(head_dim)); got %g",
                      (double)o.sm_scale);
-  if (o.kv_dtype != DK_KV_SAME && o.kv_dtype != DK_KV_FP8_E4M3)
-    return set_error(DK_EINVAL, "options.kv_dtype must be DK_KV_SAME or DK_KV_FP8_E4M3; got %d",
-                     o.kv_dtype);
+  if (o.kv_dtype != DK_KV_SAME && o.kv_dtype != DK_KV_FP8_E4M3 && o.kv_dtype != DK_KV_MXFP4)
+    return set_error(DK_EINVAL, "options.kv_dtype must be DK_KV_SAME, DK_KV_FP8_E4M3 or "
+                     "DK_KV_MXFP4; got %d", o.kv_dtype);
   if (!std::isfinite(o.k_scale) || !std::isfinite(o.v_scale) || o.k_scale < 0 ||
       o.v_scale < 0)
     return set_error(DK_EINVAL, "options.k_scale and v_scale must be finite and >= 0");
-  if (o.kv_dtype == DK_KV_SAME && (o.k_scale != 0.f || o.v_scale != 0.f))
+  if (o.kv_dtype != DK_KV_FP8_E4M3 && (o.k_scale != 0.f || o.v_scale != 0.f))
     return set_error(DK_EINVAL, "options.k_scale and v_scale apply to an fp8 cache only");
+  if (p.kv4() && (o.qk_path == 2 || (o.waves_per_group != 0 && o.waves_per_group != 4)))
+    return set_error(DK_EINVAL, "a 4-bit cache takes options.qk_path 0 or 1 and waves_per_group 0 "
+                                "or 4");
+  if (p.kv4() && (!p.need_out || p.v))
+    return set_error(DK_EUNSUPPORTED, "a 4-bit cache is one pool, read by whole calls (no separate V "
+                                      "cache, no pass 1 alone)");
   if (o.window < 0)
     return set_error(DK_EINVAL, "options.window must be >= 0 (0 = the whole sequence); got %d",
                      o.window);
@@ -247,8 +264,11 @@ int validate(const Problem& p) {
                        (long long)v);
   if (!extent_ok(p.batch, s.q_b, p.hq, s.q_h, p.head_dim, 2) ||
       (p.need_out && !extent_ok(p.batch, s.o_b, p.hq, s.o_h, p.head_dim, 2)) ||
-      !pool_ok(p.num_pages, s, kv_r, p.hkv, p.head_dim, p.kv_esize()))
+      (!p.kv4() && !pool_ok(p.num_pages, s, kv_r, p.hkv, p.head_dim, p.kv_esize())))
     return set_error(DK_EUNSUPPORTED, "q, out or kv_data spans 2^62 bytes or more");
+  if (p.kv4() && !kv4_pool_ok(p.kv, p.num_pages, s.kv_p, p.hkv, s.kv_h, p.head_dim))
+    return set_error(DK_EUNSUPPORTED, "the 4-bit cache must be 16-byte aligned, with page and head "
+                                      "strides that are multiples of 16 bytes");
   const int64_t esize = p.kv_esize();
   auto aligned16 = [](int64_t elems, int64_t es) { return (elems * es) % 16 == 0; };
   if (!aligned16(s.q_b, 2) || !aligned16(s.q_h, 2) || !aligned16(s.kv_p, esize) ||

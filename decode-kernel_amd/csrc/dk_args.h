@@ -152,6 +152,11 @@ constexpr int kGroupedWavesPerCU = 8;
 constexpr int kGroupedMinUnitsPerCU = 128;
 constexpr int kGroupedAlwaysRowBytes = 64;
 
+// 4-bit cache: wavefronts per workgroup, and per compute unit in the automatic schedules
+constexpr int kKv4Waves = 4;
+constexpr int kKv4WavesPerCU = 8;
+constexpr int kKv4StepPages = 4;     // pages that a wavefront takes at a time (2 at D = 256)
+
 // Everything a launch needs that is known on the host.
 struct Problem {
   const void* q = nullptr;
@@ -165,7 +170,8 @@ struct Problem {
   size_t workspace_bytes = 0;
   int32_t batch = 0, hq = 0, hkv = 0, head_dim = 0, page_size = 0, dtype = 0;
   int64_t num_pages = 0, num_indices = 0;
-  int32_t kv_esize() const { return opt.kv_dtype == DK_KV_FP8_E4M3 ? 1 : 2; }
+  int32_t kv_esize() const { return opt.kv_dtype == DK_KV_SAME ? 2 : 1; }   // 4 bits: of a stride
+  bool kv4() const { return opt.kv_dtype == DK_KV_MXFP4; }
   // a kv head's row of one token is at most kNarrowRowBytes
   bool narrow_rows() const { return (int64_t)head_dim * kv_esize() <= kNarrowRowBytes; }
   dk_strides st{};
@@ -235,6 +241,10 @@ bool extent_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t last, int
 // 2^62 bytes, every stride below kMaxStride.
 bool pool_ok(int64_t num_pages, const dk_strides& s, int64_t kv_r, int32_t hkv, int32_t head_dim,
              int64_t esize);
+// The same for a 4-bit pool (page and head strides in bytes): 16-byte aligned, strides multiples
+// of 16 bytes, heads of a page below 2 GiB apart.
+bool kv4_pool_ok(const void* cache, int64_t num_pages, int64_t kv_p, int32_t hkv, int64_t kv_h,
+                 int32_t head_dim);
 int64_t balanced_rows(int32_t batch, int32_t hq, int32_t hkv, int32_t head_dim);
 // Workspace of dk_decode_attention: split 1 -> 0, split > 1 -> explicit partials,
 // split 0 -> balanced partials. 0 on invalid shapes.

@@ -132,6 +132,7 @@ struct MergeArgs {
   int32_t num_indices, pairs_per_seq, heads, waves_per_pair;
   int32_t group, per, chunks, hkv;    // balanced: q head -> (head chunk, slot row)
   int32_t seg_cost;                   // balanced: pass 1's seg_cost (0: equal page ranges)
+  int32_t keep_nan;                   // a row whose sum is NaN is NaN (0: zeros, as for an empty one)
   const float* sinks;                 // attention sinks: one fp32 logit per q head, or null
 };
 
@@ -1778,8 +1779,9 @@ __device__ __forceinline__ void merge_row(const MergeArgs& m, int row, const flo
   // zero output, when no slot saw a token)
   if (m.sinks) L += __builtin_amdgcn_exp2f((m.sinks[qh] - M) * kLog2e);
   uint8_t* op = m.out + (int64_t)b * m.o_b + (int64_t)qh * m.o_h + 2 * lane * E;
+  const bool live = L > 0.f || (m.keep_nan && L != L);
 #pragma unroll
-  for (int e = 0; e < E; ++e) T::store(op + 2 * e, L > 0.f ? acc[e] / L : 0.f);
+  for (int e = 0; e < E; ++e) T::store(op + 2 * e, live ? acc[e] / L : 0.f);
 }
 
 template <class T, int D>

@@ -110,14 +110,17 @@ PyObject* decode_impl(PyObject* const* args) {
 
   const at::Device dev = q.device();
   const bool f16 = q.scalar_type() == at::kHalf, kv8 = k->scalar_type() == at::kFloat8_e4m3fn;
+  // a 4-bit cache: uint8 (num_pages, num_kv_heads, 17 * head_dim)
+  const bool kv4 = k->scalar_type() == at::kByte && !pair;
   if (!dev.is_cuda() || q.dim() != 3 || !(f16 || q.scalar_type() == at::kBFloat16) ||
-      !(kv8 || k->scalar_type() == q.scalar_type()) || k->device() != dev)
+      !(kv8 || kv4 || k->scalar_type() == q.scalar_type()) || k->device() != dev)
     Py_RETURN_NONE;
-  const int kd = pair ? 4 : 5;
-  if (k->dim() != kd || (!pair && k->size(1) != 2)) Py_RETURN_NONE;
+  const int kd = pair ? 4 : kv4 ? 3 : 5;
+  if (k->dim() != kd || (kd == 5 && k->size(1) != 2)) Py_RETURN_NONE;
   const int64_t batch = q.size(0), hq = q.size(1), d = q.size(2);
-  const int64_t page = k->size(kd - 3), hkv = k->size(kd - 2);
-  if (page != 16 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || k->size(kd - 1) != d ||
+  const int64_t page = kv4 ? 16 : k->size(kd - 3), hkv = k->size(kd - 2);
+  if (page != 16 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv ||
+      k->size(kd - 1) != (kv4 ? 17 * d : d) ||
       (d != 64 && d != 128 && d != 256) || batch > INT32_MAX || hq > INT32_MAX ||
       q.stride(2) != 1 || k->stride(kd - 1) != 1)
     Py_RETURN_NONE;
@@ -149,6 +152,7 @@ PyObject* decode_impl(PyObject* const* args) {
     o.k_scale = scale[0];
     o.v_scale = scale[1];
   }
+  if (kv4) o.kv_dtype = DK_KV_MXFP4;
   if (args[kSinks] != Py_None) {
     const at::Tensor* s = tensor_arg(args[kSinks]);
     if (!s || s->scalar_type() != at::kFloat || s->dim() != 1 || s->size(0) != hq ||
@@ -214,8 +218,8 @@ PyObject* decode_impl(PyObject* const* args) {
   s.q_b = q.stride(0);
   s.q_h = q.stride(1);
   s.kv_p = k->stride(0);
-  s.kv_r = pair ? 0 : k->stride(1);
-  s.kv_s = k->stride(kd - 3);
+  s.kv_r = pair || kv4 ? 0 : k->stride(1);
+  s.kv_s = kv4 ? 0 : k->stride(kd - 3);
   s.kv_h = k->stride(kd - 2);
   s.o_b = out.stride(0);
   s.o_h = out.stride(1);

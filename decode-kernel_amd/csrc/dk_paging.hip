@@ -1,6 +1,6 @@
 // dk_paging.hip — page tables for the decode path (C ABI in include/dk_decode.h):
 // dk_build_page_table from a token-slot map, dk_expand_page_table from a table of larger
-// pages.
+// pages, dk_grow_block_tables from request lengths.
 //
 // Serving frameworks (SGLang's ReqToTokenPool) keep, per request, the cache slot of every
 // token: req_to_token[req][t]. With a paged allocator of 16-token pages, token t of a
@@ -165,8 +165,159 @@ __global__ __launch_bounds__(kThreads) void dk_expand_pages(ExpandArgs a) {
   }
 }
 
+struct GrowArgs {
+  int32_t* table;              // (num_rows, max_blocks): page ids of each row's 16-token blocks
+  int64_t stride;              // elements between rows
+  int64_t num_rows;
+  int32_t max_blocks;
+  const void *rows, *cached, *added;   // per request, int32 or int64
+  int32_t rows64, cached64, added64;
+  const int32_t* pages;        // page ids to hand out, in order
+  int64_t num_pages;
+  int32_t batch;
+  int32_t* kv_indptr;
+  int32_t* kv_indices;
+  int64_t capacity;
+  int32_t* kv_last;
+  int32_t* q_indptr;
+  int32_t* slots;
+  int32_t* positions;
+  int64_t num_tokens;          // entries of slots and positions
+};
+
+__device__ __forceinline__ int64_t entry64(const void* p, int32_t wide, int64_t i) {
+  return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// What request b holds: its row (-1: it has no pages), the blocks of its cached tokens and of all
+// its tokens, its new tokens. A row outside the table, a negative length and a length beyond the
+// row's blocks leave it without pages; its new tokens keep their places, without slots.
+struct GrowRequest {
+  int64_t row, cached, added, before, blocks;
+};
+__device__ __forceinline__ GrowRequest grow_request(const GrowArgs& a, int b) {
+  GrowRequest r;
+  r.row = entry64(a.rows, a.rows64, b);
+  r.cached = entry64(a.cached, a.cached64, b);
+  const int64_t n = entry64(a.added, a.added64, b);
+  const int64_t most = (int64_t)a.max_blocks * kPageSize;
+  r.added = min(max(n, (int64_t)0), (int64_t)INT32_MAX);
+  const bool ok = r.row >= 0 && r.row < a.num_rows && n >= 0 && r.cached >= 0 && r.cached <= most &&
+                  n <= most - r.cached;
+  if (!ok) r.row = -1;
+  r.before = ok ? (r.cached + kPageSize - 1) / kPageSize : 0;
+  r.blocks = ok ? (r.cached + n + kPageSize - 1) / kPageSize : 0;
+  return r;
+}
+
+// Workgroups (request b, slice of its blocks and new tokens). A request's places in the three
+// outputs are sums over the requests before it, recomputed per workgroup as dk_page_table does:
+// the blocks (kv_indices), the blocks that are new (the ids handed out), the new tokens. A new
+// block's id comes straight from `pages`, so no workgroup reads what another writes (requests
+// name different rows). One launch in place of some 30 small ones, bound by its latency (lengths,
+// rows and table, three dependent reads).
+__global__ __launch_bounds__(kThreads) void dk_grow_tables(GrowArgs a) {
+  __shared__ int64_t partial[3][kThreads / 64];
+  const int b = blockIdx.x;
+  const int tid = threadIdx.x;
+  const GrowRequest r = grow_request(a, b);
+  int64_t sum[3] = {0, 0, 0};
+  for (int j = tid; j < b; j += kThreads) {
+    const GrowRequest x = grow_request(a, j);
+    sum[0] += x.blocks;
+    sum[1] += x.blocks - x.before;
+    sum[2] += x.added;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    for (int o = 32; o > 0; o >>= 1) sum[i] += __shfl_xor(sum[i], o, 64);
+    if ((tid & 63) == 0) partial[i][tid >> 6] = sum[i];
+  }
+  __syncthreads();
+  int64_t at[3] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) at[i] += partial[i][w];
+
+  if (tid == 0 && blockIdx.y == 0) {
+    if (b == 0) a.kv_indptr[0] = a.q_indptr[0] = 0;
+    // the true offsets, saturated at int32's range
+    a.kv_indptr[b + 1] = (int32_t)min(at[0] + r.blocks, (int64_t)INT32_MAX);
+    a.q_indptr[b + 1] = (int32_t)min(at[2] + r.added, (int64_t)INT32_MAX);
+    a.kv_last[b] = r.blocks > 0 ? (int32_t)(r.cached + r.added - (r.blocks - 1) * kPageSize) : 0;
+  }
+  int32_t* row = a.table + max(r.row, (int64_t)0) * a.stride;
+  const int64_t first = blockIdx.y * kThreads + tid, step = (int64_t)gridDim.y * kThreads;
+  auto fresh = [&](int64_t p) -> int32_t {                   // id of the request's new block p
+    const int64_t i = at[1] + p - r.before;
+    return i < a.num_pages ? a.pages[i] : -1;
+  };
+  for (int64_t p = first; p < r.blocks; p += step) {
+    int32_t id;
+    if (p >= r.before) row[p] = id = fresh(p);
+    else id = row[p];
+    if (at[0] + p < a.capacity) a.kv_indices[at[0] + p] = id;
+  }
+  for (int64_t i = first; i < r.added && at[2] + i < a.num_tokens; i += step) {
+    int32_t slot = -1, pos = 0;
+    if (r.row >= 0) {
+      const int64_t t = r.cached + i, p = t / kPageSize;
+      const int32_t id = p >= r.before ? fresh(p) : row[p];
+      pos = (int32_t)t;
+      if (id >= 0 && id <= (INT32_MAX - (kPageSize - 1)) / kPageSize)
+        slot = id * kPageSize + (int32_t)(t % kPageSize);
+    }
+    a.slots[at[2] + i] = slot;
+    a.positions[at[2] + i] = pos;
+  }
+  if (b == a.batch - 1)                                      // rows behind the last new token
+    for (int64_t i = at[2] + r.added + first; i < a.num_tokens; i += step) {
+      a.slots[i] = -1;
+      a.positions[i] = 0;
+    }
+}
+
 }  // namespace
 }  // namespace dk
+
+extern "C" int dk_grow_block_tables(int32_t* block_table, int64_t table_stride, int64_t num_rows,
+                                    int32_t max_blocks, const void* rows, int32_t rows_int64,
+                                    const void* cached_lens, int32_t cached_int64,
+                                    const void* new_lens, int32_t new_int64,
+                                    const int32_t* new_pages, int64_t num_new_pages, int32_t batch,
+                                    int32_t* kv_indptr, int32_t* kv_indices, int64_t capacity,
+                                    int32_t* kv_last_page_len, int32_t* q_indptr, int32_t* slots,
+                                    int32_t* positions, int64_t num_tokens, void* hip_stream) {
+  using namespace dk;
+  clear_error();
+  if (batch < 0 || num_rows < 0 || max_blocks < 0 || num_new_pages < 0 || capacity < 0 ||
+      num_tokens < 0 || table_stride < 0 || num_tokens > INT32_MAX || capacity > INT32_MAX)
+    return set_error(DK_EINVAL, "dk_grow_block_tables: negative or too large a size");
+  if (max_blocks > (INT32_MAX - kPageSize) / kPageSize)
+    return set_error(DK_EINVAL, "dk_grow_block_tables: max_blocks must be below 2^27");
+  if (table_stride >= kMaxStride || num_rows >= kMaxStride ||
+      (__int128)num_rows * table_stride >= ((__int128)1 << 60))
+    return set_error(DK_EUNSUPPORTED, "dk_grow_block_tables: the table spans 2^62 bytes or more");
+  if (num_rows > 1 && table_stride < max_blocks)
+    return set_error(DK_EINVAL, "dk_grow_block_tables: rows of the table overlap");
+  if (batch == 0) return DK_OK;
+  if (!rows || !cached_lens || !new_lens || !kv_indptr || !kv_last_page_len || !q_indptr ||
+      (num_rows > 0 && max_blocks > 0 && !block_table) || (num_new_pages > 0 && !new_pages) ||
+      (capacity > 0 && !kv_indices) || (num_tokens > 0 && (!slots || !positions)))
+    return set_error(DK_ENULL, "dk_grow_block_tables: NULL pointer");
+  GrowArgs a{block_table, table_stride, num_rows, max_blocks, rows, cached_lens, new_lens,
+             rows_int64 != 0, cached_int64 != 0, new_int64 != 0, new_pages, num_new_pages, batch,
+             kv_indptr, kv_indices, capacity, kv_last_page_len, q_indptr, slots, positions,
+             num_tokens};
+  void* args[] = {&a};
+  const hipError_t e = hipLaunchKernel((const void*)dk_grow_tables,
+                                       dim3(batch, slices(std::max(capacity, num_tokens), batch)),
+                                       dim3(kThreads), args, 0,
+                                       static_cast<hipStream_t>(hip_stream));
+  if (e != hipSuccess) return set_error((int)e, "block-table launch: %s", hipGetErrorString(e));
+  return DK_OK;
+}
 
 extern "C" int dk_expand_page_table(const int32_t* kv_indptr, const int32_t* kv_indices,
                                     const int32_t* kv_last_page_len, int32_t batch,

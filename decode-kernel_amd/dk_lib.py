@@ -19,6 +19,7 @@ DK_F16 = 0
 DK_BF16 = 1
 DK_KV_SAME = 0
 DK_KV_FP8_E4M3 = 2
+DK_KV_MXFP4 = 3
 ABI_VERSION = 3
 STATIC_SCRATCH_BYTES = 32 << 20     # DK_STATIC_SCRATCH_BYTES: dk_decode_attention_noalloc
 
@@ -105,6 +106,15 @@ SIGNATURES = {
                                         _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I32,
                                         ctypes.c_float, ctypes.c_float,
                                         ctypes.POINTER(DkStrides), _P]),
+    "dk_grow_block_tables": (ctypes.c_int, [_P, _I64, _I64, _I32, _P, _I32, _P, _I32, _P, _I32, _P,
+                                            _I64, _I32, _P, _P, _I64, _P, _P, _P, _P, _I64, _P]),
+    "dk_kv4_write": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _P, _I32, _P, _I32, _P, _I32, _I64,
+                                    _I32, _I32, _I32, _I64, _I32, ctypes.POINTER(DkStrides), _P]),
+    "dk_kv4_append": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I32, _I32,
+                                     _I32, _I32, _I32, _I64, _I64, _I32,
+                                     ctypes.POINTER(DkStrides), _P]),
+    "dk_kv4_read": (ctypes.c_int, [_P, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _I64, _I32, _I32,
+                                   _I64, _I32, _P]),
     "dk_extend_workspace_bytes": (_SZ, [_I32, ctypes.POINTER(_I32), ctypes.POINTER(_I32), _I32,
                                         _I32, _I32, _I32]),
     "dk_extend_attention": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, ctypes.POINTER(_I32),

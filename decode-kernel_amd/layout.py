@@ -147,6 +147,40 @@ def synthesize_paged(batch: int, context_lengths: Union[int, Sequence[int]], num
             torch.tensor(last, dtype=torch.int32, device=device), layout)
 
 
+# ---- the 4-bit cache (OCP MXFP4; DK_KV_MXFP4 in include/dk_decode.h describes its bytes)
+
+KV4_BYTES_PER_DIM = 17      # of a page block: 16 tokens' K and V codes and their scales
+
+
+def alloc_kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int,
+                    device: Union[str, torch.device] = "cuda") -> torch.Tensor:
+    """A 4-bit paged cache, all zeros: uint8 (num_pages, num_kv_heads, 17 * head_dim), one block of
+    16 tokens' K and V per page and kv head. decode_attention, append_kv, write_kv4, read_kv4 and
+    extend_attention_kv4 take it (or a view of some of its kv heads or pages)."""
+    if head_dim not in (64, 128, 256):
+        raise LayoutError(f"head_dim must be 64, 128 or 256; got {head_dim}")
+    return torch.zeros(num_pages, num_kv_heads, KV4_BYTES_PER_DIM * head_dim, dtype=torch.uint8,
+                       device=device)
+
+
+def is_kv4(kv_data) -> bool:
+    """Whether kv_data is a 4-bit cache: a 3-D uint8 tensor."""
+    return isinstance(kv_data, torch.Tensor) and kv_data.dtype == torch.uint8 and kv_data.dim() == 3
+
+
+def kv4_head_dim(cache: torch.Tensor) -> int:
+    """head_dim of a 4-bit cache; raises LayoutError on a malformed one."""
+    if not is_kv4(cache):
+        raise LayoutError("a 4-bit cache is a uint8 tensor (num_pages, num_kv_heads, 17 * head_dim)")
+    d, rest = divmod(cache.shape[2], KV4_BYTES_PER_DIM)
+    if rest or d not in (64, 128, 256):
+        raise LayoutError(f"a 4-bit cache's page block has 17 * head_dim bytes (head_dim 64, 128 or "
+                          f"256); got {cache.shape[2]}")
+    if cache.stride(2) != 1:
+        raise LayoutError("the bytes of a 4-bit cache's page block must be contiguous")
+    return d
+
+
 def ragged_lengths(batch: int, lo: int, hi: int, seed: int = 0):
     """Per-sequence context lengths uniform in [lo, hi] (seeded, CPU)."""
     g = torch.Generator(device="cpu")

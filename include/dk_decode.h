@@ -49,6 +49,16 @@ typedef enum { DK_F16 = 0, DK_BF16 = 1 } dk_dtype;
  * counterpart in the reference (fp16 cache only). */
 #define DK_KV_SAME 0
 #define DK_KV_FP8_E4M3 2
+/* A 4-bit cache (OCP MXFP4): kv_data is a pool of page blocks, one per (page, kv head), kv_p and
+ * kv_h BYTES apart (kv_r and kv_s are not read), each 17 * head_dim bytes for 16 tokens: E2M1
+ * codes, two per byte (the even dim in the low nibble), and E8M0 scales, one per 32 dims of a row
+ * (a value is code * 2^(scale - 127), NaN where the scale is 255):
+ *   K code byte of (token t, dim d)   t * D/2 + d/2
+ *   V code byte                       8 D + (d/W) 8 W + (t/4) 2 W + (d%W / (W/16)) W/8
+ *                                       + (t%4) W/32 + (d % (W/16)) / 2,    W = min(D, 128)
+ *   K scale byte of block b           16 D + 16 b + t;     V scale byte: D/2 further
+ * The pool is 16-byte aligned and kv_p, kv_h are multiples of 16. No counterpart in the reference. */
+#define DK_KV_MXFP4 3
 
 /* Error codes (< 0). */
 enum {
@@ -96,7 +106,9 @@ typedef struct {
   float sm_scale;          /* softmax scale applied to q.k; 0 = 1/sqrt(head_dim), the
                               reference's fixed scale (attention_ext.cu:79-80)             */
   int32_t kv_dtype;        /* DK_KV_SAME (0): the cache has q's type; DK_KV_FP8_E4M3: fp8
-                              (strides still in elements, now bytes)                      */
+                              (strides still in elements, now bytes); DK_KV_MXFP4: 4 bits
+                              (qk_path 0 or 1, waves_per_group 0 or 4, no separate V cache, no
+                              dk_decode_partials; a NaN in the cache gives NaN outputs)    */
   float k_scale;           /* fp8 cache: K = k_scale * stored value (0 = 1); must be 0
                               for a cache of q's type                                     */
   float v_scale;           /* fp8 cache: V = v_scale * stored value (0 = 1); likewise     */
@@ -293,6 +305,29 @@ int dk_expand_page_table(const int32_t* kv_indptr, const int32_t* kv_indices,
                          int32_t* out_indptr, int32_t* out_indices, int64_t capacity,
                          int32_t* out_last_page_len, void* hip_stream);
 
+/* Block tables, page table and slot map of a step from request lengths, in one launch. Request b
+ * has row rows[b] of block_table (num_rows rows of max_blocks page ids, table_stride int32 apart;
+ * entry i holds its tokens 16 i .. 16 i + 15), cached_lens[b] tokens in the cache and new_lens[b] to
+ * come (each array int32, or int64 where its flag is nonzero). It needs ceil((cached + new) / 16)
+ * - ceil(cached / 16) new blocks; the requests' new blocks, in order, take new_pages[0], [1], ..
+ * (-1 past num_new_pages). Writes
+ *   block_table                    the new entries, nothing else;
+ *   kv_indptr, kv_indices,         the CSR page table of cached + new tokens, as
+ *   kv_last_page_len               dk_build_page_table's (at most `capacity` indices);
+ *   q_indptr (batch + 1)           the requests' new tokens among all new tokens;
+ *   slots, positions (num_tokens)  of each new token, 16 * page + position % 16 (-1 without a page)
+ *                                  and its index in its request; -1 and 0 behind the last one.
+ * The rows of a batch are distinct. A row outside the table, a negative length and one beyond
+ * 16 * max_blocks leave a request without pages (its new tokens keep their places, slots -1).
+ * Device pointers; enqueued on hip_stream. No counterpart in the reference. */
+int dk_grow_block_tables(int32_t* block_table, int64_t table_stride, int64_t num_rows,
+                         int32_t max_blocks, const void* rows, int32_t rows_int64,
+                         const void* cached_lens, int32_t cached_int64, const void* new_lens,
+                         int32_t new_int64, const int32_t* new_pages, int64_t num_new_pages,
+                         int32_t batch, int32_t* kv_indptr, int32_t* kv_indices, int64_t capacity,
+                         int32_t* kv_last_page_len, int32_t* q_indptr, int32_t* slots,
+                         int32_t* positions, int64_t num_tokens, void* hip_stream);
+
 /* Cache write before a decode step: for every sequence b, the new token is the last one
  * the page table describes (page kv_indices[kv_indptr[b+1] - 1], slot
  * kv_last_page_len[b] - 1; grow the table first). Writes its K row rotated by rotary
@@ -327,6 +362,37 @@ int dk_append_kv_fp8(void* q, const void* k_new, const void* v_new, int64_t new_
                      int32_t head_dim, int32_t page_size, int64_t num_pages,
                      int64_t num_indices, int32_t dtype, float k_scale, float v_scale,
                      const dk_strides* strides, void* hip_stream);
+
+/* Write of any number of tokens into a 4-bit cache (DK_KV_MXFP4): token t's K row (rotated as in
+ * dk_append_kv, at positions[t]) and V row for all kv heads go to slot slots[t] = 16 * page +
+ * token of the page; a slot outside [0, 16 * num_pages) writes nothing. Slots of one call are
+ * distinct. q (optional) is rotated in place for every token. k_new / v_new / q have type `dtype`;
+ * `strides` gives q_b, q_h (elements) and kv_p, kv_h (bytes). Each block of 32 dims is held as codes
+ * times the power of two that puts its largest magnitude in [3.5, 7): to the nearest code, ties to
+ * the even one; a block with a NaN or an infinity reads as NaN. Angles are position * inv_freq
+ * without the rounding of an fp32 product. inv_freq NULL: no rotation. */
+int dk_kv4_write(void* q, const void* k_new, const void* v_new, int64_t new_t, int64_t new_h,
+                 void* cache, const void* slots, int32_t slots_int64, const void* positions,
+                 int32_t positions_int64, const float* inv_freq, int32_t rope_style,
+                 int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                 int64_t num_pages, int32_t dtype, const dk_strides* strides, void* hip_stream);
+
+/* dk_append_kv into a 4-bit cache: one token per sequence, in the last slot of its page table (a
+ * page id outside the pool writes nothing). */
+int dk_kv4_append(void* q, const void* k_new, const void* v_new, int64_t new_b, int64_t new_h,
+                  void* cache, const int32_t* kv_indptr, const int32_t* kv_indices,
+                  const int32_t* kv_last_page_len, const int32_t* positions,
+                  const float* inv_freq, int32_t rope_style, int32_t batch, int32_t num_q_heads,
+                  int32_t num_kv_heads, int32_t head_dim, int64_t num_pages, int64_t num_indices,
+                  int32_t dtype, const dk_strides* strides, void* hip_stream);
+
+/* The rows that a 4-bit cache holds in the given slots, as `dtype` values (exact in bf16; in fp16
+ * beyond its range infinite), zeros for a slot outside the pool: k_out / v_out (num_tokens,
+ * num_kv_heads, head_dim), out_t / out_h elements apart. kv_p, kv_h in bytes. */
+int dk_kv4_read(const void* cache, int64_t kv_p, int64_t kv_h, const void* slots,
+                int32_t slots_int64, void* k_out, void* v_out, int64_t out_t, int64_t out_h,
+                int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
+                int32_t dtype, void* hip_stream);
 
 /* Element strides of dk_extend_attention: q / out rows (one per new token) and heads, K and V
  * pool token slots and kv heads; the head_dim stride is 1 everywhere. */
