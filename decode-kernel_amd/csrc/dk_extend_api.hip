@@ -47,6 +47,85 @@ hipError_t merge(const ExtendArgs& a, int64_t tokens, int d, hipStream_t stream)
   return launch_merge<T>(m, d, false, stream);
 }
 
+// Sizes of each request, in range of the map (rows of `width` entries' tokens) and of q; *first:
+// the new tokens in all.
+int check_requests(int32_t batch, const int32_t* rows, const int32_t* new_lens,
+                   const int32_t* all_lens, int64_t num_rows, int32_t group, int64_t num_tokens,
+                   int64_t width, int64_t* first) {
+  *first = 0;
+  for (int32_t b = 0; b < batch; ++b) {
+    if (new_lens[b] < 0 || all_lens[b] < new_lens[b] || all_lens[b] > INT32_MAX - 1024 ||
+        (int64_t)new_lens[b] * group > INT32_MAX - 1024)
+      return set_error(DK_EINVAL, "request %d: %d new of %d tokens", b, new_lens[b], all_lens[b]);
+    if (rows[b] < 0 || rows[b] >= num_rows || all_lens[b] > width)
+      return set_error(DK_EINVAL, "request %d: row %d or its length exceeds the map", b, rows[b]);
+    *first += new_lens[b];
+  }
+  if (*first > num_tokens)
+    return set_error(DK_EINVAL, "%lld new tokens in q rows for %lld", (long long)*first,
+                     (long long)num_tokens);
+  return DK_OK;
+}
+
+// The split of the keys, its workspace and the launches of a call whose arguments are checked;
+// first: its new tokens.
+int launch_extend(ExtendArgs& a, int pool, const int32_t* rows, const int32_t* new_lens,
+                  const int32_t* all_lens, void* workspace, size_t workspace_bytes, int32_t batch,
+                  int64_t first, int32_t head_dim, int32_t dtype, bool cap, void* hip_stream) {
+  // without a workspace for the partials the keys are not split
+  a.split = extend_split(batch, new_lens, all_lens, a.hkv, a.group, a.window);
+  if (a.split > 1) {
+    size_t off_o, off_m, off_l, total;
+    partials_layout_rows(first * (a.hkv * a.group) * a.split, head_dim, &off_o, &off_m, &off_l, &total);
+    if (!workspace || workspace_bytes < total || (uintptr_t)workspace % 256 != 0) {
+      a.split = 1;
+    } else {
+      uint8_t* ws = static_cast<uint8_t*>(workspace);
+      a.part_o = reinterpret_cast<float*>(ws + off_o);
+      a.part_m = reinterpret_cast<float*>(ws + off_m);
+      a.part_l = reinterpret_cast<float*>(ws + off_l);
+    }
+  }
+  const bool bf16 = dtype == DK_BF16;
+  const void* fn = head_dim == 64    ? extend_symbol<64>(bf16, pool, cap)
+                   : head_dim == 128 ? extend_symbol<128>(bf16, pool, cap)
+                                     : extend_symbol<256>(bf16, pool, cap);
+  // kExtendMaxReqs requests per launch: their sizes travel as kernel arguments, so a call
+  // copies nothing to the device
+  int32_t b = 0;
+  int64_t q0 = 0;
+  while (b < batch) {
+    int32_t n = 0;
+    int64_t tiles = 0;
+    for (; b < batch && n < kExtendMaxReqs; ++b) {
+      if (new_lens[b] == 0) continue;
+      const int64_t t = ((int64_t)new_lens[b] * a.group + kExtendRows - 1) / kExtendRows;
+      if ((tiles + t) * a.hkv > INT32_MAX) {
+        if (n == 0) return set_error(DK_EUNSUPPORTED, "request %d has too many new tokens", b);
+        break;
+      }
+      a.req[n++] = ExtendReq{rows[b], (int32_t)q0, new_lens[b], all_lens[b], (int32_t)tiles};
+      tiles += t;
+      q0 += new_lens[b];
+    }
+    if (n == 0) break;
+    a.num_reqs = n;
+    a.tiles = (int32_t)tiles;
+    void* args[] = {&a};
+    const hipError_t e =
+        hipLaunchKernel(fn, dim3((uint32_t)(tiles * a.hkv), a.split), dim3(kExtendThreads), args, 0,
+                        static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return set_error((int)e, "extend launch: %s", hipGetErrorString(e));
+  }
+  if (a.split > 1) {
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e =
+        bf16 ? merge<BF16>(a, first, head_dim, st) : merge<F16>(a, first, head_dim, st);
+    if (e != hipSuccess) return set_error((int)e, "extend merge launch: %s", hipGetErrorString(e));
+  }
+  return DK_OK;
+}
+
 }  // namespace
 }  // namespace dk
 
@@ -114,17 +193,9 @@ extern "C" int dk_extend_attention(
     return set_error(DK_EUNSUPPORTED, "pool slots must be less than 2^31 bytes apart");
   const int32_t group = num_q_heads / num_kv_heads;
   int64_t first = 0;
-  for (int32_t b = 0; b < batch; ++b) {
-    if (new_lens[b] < 0 || all_lens[b] < new_lens[b] || all_lens[b] > INT32_MAX - 1024 ||
-        (int64_t)new_lens[b] * group > INT32_MAX - 1024)
-      return set_error(DK_EINVAL, "request %d: %d new of %d tokens", b, new_lens[b], all_lens[b]);
-    if (rows[b] < 0 || rows[b] >= num_rows || (num_rows > 1 && all_lens[b] > req_stride))
-      return set_error(DK_EINVAL, "request %d: row %d or its length exceeds the map", b, rows[b]);
-    first += new_lens[b];
-  }
-  if (first > num_tokens)
-    return set_error(DK_EINVAL, "%lld new tokens in q rows for %lld", (long long)first,
-                     (long long)num_tokens);
+  if (const int rc = check_requests(batch, rows, new_lens, all_lens, num_rows, group, num_tokens,
+                                    num_rows > 1 ? req_stride : INT32_MAX, &first))
+    return rc;
   if (first == 0) return DK_OK;
   if (!q || !k_pool || !v_pool || !req_to_token || !out)
     return set_error(DK_ENULL, "dk_extend_attention: NULL pointer");
@@ -154,56 +225,79 @@ extern "C" int dk_extend_attention(
   a.cap_in = logit_cap != 0.f ? score_scale / logit_cap : 0.f;
   a.cap_out = kLog2e * logit_cap;
   a.vscale = v_scale;
-  // without a workspace for the partials the keys are not split
-  a.split = extend_split(batch, new_lens, all_lens, num_kv_heads, group, window);
-  if (a.split > 1) {
-    size_t off_o, off_m, off_l, total;
-    partials_layout_rows(first * num_q_heads * a.split, head_dim, &off_o, &off_m, &off_l, &total);
-    if (!workspace || workspace_bytes < total || (uintptr_t)workspace % 256 != 0) {
-      a.split = 1;
-    } else {
-      uint8_t* ws = static_cast<uint8_t*>(workspace);
-      a.part_o = reinterpret_cast<float*>(ws + off_o);
-      a.part_m = reinterpret_cast<float*>(ws + off_m);
-      a.part_l = reinterpret_cast<float*>(ws + off_l);
-    }
-  }
-  const bool bf16 = dtype == DK_BF16, kv8 = kes == 1, cap = logit_cap != 0.f;
-  const void* fn = head_dim == 64    ? extend_symbol<64>(bf16, kv8, cap)
-                   : head_dim == 128 ? extend_symbol<128>(bf16, kv8, cap)
-                                     : extend_symbol<256>(bf16, kv8, cap);
-  // kExtendMaxReqs requests per launch: their sizes travel as kernel arguments, so a call
-  // copies nothing to the device
-  int32_t b = 0;
-  int64_t q0 = 0;
-  while (b < batch) {
-    int32_t n = 0;
-    int64_t tiles = 0;
-    for (; b < batch && n < kExtendMaxReqs; ++b) {
-      if (new_lens[b] == 0) continue;
-      const int64_t t = ((int64_t)new_lens[b] * group + kExtendRows - 1) / kExtendRows;
-      if ((tiles + t) * num_kv_heads > INT32_MAX) {
-        if (n == 0) return set_error(DK_EUNSUPPORTED, "request %d has too many new tokens", b);
-        break;
-      }
-      a.req[n++] = ExtendReq{rows[b], (int32_t)q0, new_lens[b], all_lens[b], (int32_t)tiles};
-      tiles += t;
-      q0 += new_lens[b];
-    }
-    if (n == 0) break;
-    a.num_reqs = n;
-    a.tiles = (int32_t)tiles;
-    void* args[] = {&a};
-    const hipError_t e =
-        hipLaunchKernel(fn, dim3((uint32_t)(tiles * num_kv_heads), a.split), dim3(kExtendThreads), args, 0,
-                        static_cast<hipStream_t>(hip_stream));
-    if (e != hipSuccess) return set_error((int)e, "extend launch: %s", hipGetErrorString(e));
-  }
-  if (a.split > 1) {
-    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const hipError_t e =
-        bf16 ? merge<BF16>(a, first, head_dim, st) : merge<F16>(a, first, head_dim, st);
-    if (e != hipSuccess) return set_error((int)e, "extend merge launch: %s", hipGetErrorString(e));
-  }
-  return DK_OK;
+  return launch_extend(a, kes == 1 ? kPoolFp8 : kPoolSame, rows, new_lens, all_lens, workspace,
+                       workspace_bytes, batch, first, head_dim, dtype, logit_cap != 0.f, hip_stream);
+}
+
+extern "C" int dk_extend_attention_kv4(
+    const void* q, const void* cache, int64_t kv_p, int64_t kv_h, const int32_t* block_table,
+    int64_t table_stride, int64_t num_rows, int32_t max_blocks, const int32_t* rows,
+    const int32_t* new_lens, const int32_t* all_lens, void* out, void* workspace,
+    size_t workspace_bytes, int32_t batch, int64_t num_tokens, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int64_t num_pages, int32_t dtype,
+    const dk_extend_strides* strides, float score_scale, float logit_cap, int32_t window,
+    const float* sinks, void* hip_stream) {
+  using namespace dk;
+  clear_error();
+  if (!strides) return set_error(DK_ENULL, "strides must be non-NULL");
+  if (batch < 0 || num_tokens < 0 || num_tokens > INT32_MAX || num_q_heads <= 0 ||
+      num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || window < 0 || num_rows < 0 ||
+      num_rows > INT32_MAX || num_pages < 0 || num_pages > INT32_MAX || table_stride < 0 ||
+      table_stride >= kMaxStride || max_blocks < 0 || (num_rows > 1 && max_blocks > table_stride))
+    return set_error(DK_EINVAL, "dk_extend_attention_kv4: bad sizes");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return set_error(DK_EINVAL, "head_dim must be 64, 128 or 256; got %d", head_dim);
+  if (dtype != DK_F16 && dtype != DK_BF16)
+    return set_error(DK_EINVAL, "dtype must be DK_F16 or DK_BF16; got %d", dtype);
+  if (!std::isfinite(score_scale) || !(score_scale > 0.f) || !std::isfinite(logit_cap))
+    return set_error(DK_EINVAL, "score_scale must be finite and > 0, logit_cap finite");
+  if (batch == 0) return DK_OK;
+  if (!rows || !new_lens || !all_lens)
+    return set_error(DK_ENULL, "dk_extend_attention_kv4: NULL pointer");
+  const dk_extend_strides& s = *strides;
+  if (!extent_ok(num_tokens, s.q_b, num_q_heads, s.q_h, head_dim, 2) ||
+      !extent_ok(num_tokens, s.o_b, num_q_heads, s.o_h, head_dim, 2))
+    return set_error(DK_EUNSUPPORTED, "strides must be non-negative and below 2^40 elements");
+  for (int64_t b : {s.q_b, s.q_h, s.o_b, s.o_h, (int64_t)((uintptr_t)q % 16) / 2,
+                    (int64_t)((uintptr_t)out % 16) / 2})
+    if (b % 8 != 0 || (uintptr_t)q % 2 || (uintptr_t)out % 2)
+      return set_error(DK_EUNSUPPORTED, "q and out must be 16-byte aligned, and their strides "
+                                        "multiples of 16 bytes");
+  if (!kv4_pool_ok(cache, num_pages, kv_p, num_kv_heads, kv_h, head_dim))
+    return set_error(DK_EUNSUPPORTED, "the 4-bit cache must be 16-byte aligned, with page and head "
+                                      "strides that are non-negative multiples of 16 bytes");
+  const int32_t group = num_q_heads / num_kv_heads;
+  int64_t first = 0;
+  if (const int rc = check_requests(batch, rows, new_lens, all_lens, num_rows, group, num_tokens,
+                                    (int64_t)max_blocks * kPageSize, &first))
+    return rc;
+  if (first == 0) return DK_OK;
+  if (!q || !cache || !block_table || !out)
+    return set_error(DK_ENULL, "dk_extend_attention_kv4: NULL pointer");
+  if (num_pages == 0) return set_error(DK_EINVAL, "the page pool is empty");
+
+  ExtendArgs a{};
+  a.q = static_cast<const uint8_t*>(q);
+  a.k = static_cast<const uint8_t*>(cache);
+  a.req_to_token = block_table;
+  a.out = static_cast<uint8_t*>(out);
+  a.sinks = sinks;
+  a.q_b = s.q_b * 2;
+  a.q_h = s.q_h * 2;
+  a.o_b = s.o_b * 2;
+  a.o_h = s.o_h * 2;
+  a.k_h = kv_h;
+  a.kv_p = kv_p;
+  a.req_stride = table_stride;
+  a.group = group;
+  a.hkv = num_kv_heads;
+  a.window = window;
+  a.num_slots = (uint32_t)num_pages;
+  constexpr float kStage = 1 << kKv4StageExp;
+  a.kscale = kLog2e * score_scale * kStage;
+  a.cap_in = logit_cap != 0.f ? score_scale * kStage / logit_cap : 0.f;
+  a.cap_out = kLog2e * logit_cap;
+  a.vscale = kStage;
+  return launch_extend(a, kPoolKv4, rows, new_lens, all_lens, workspace, workspace_bytes, batch, first,
+                       head_dim, dtype, logit_cap != 0.f, hip_stream);
 }

@@ -122,6 +122,12 @@ SIGNATURES = {
                                            _I32, _I64, _I32, _I32, _I32, _I64, _I32, _I32,
                                            ctypes.POINTER(DkExtendStrides), ctypes.c_float,
                                            ctypes.c_float, ctypes.c_float, _I32, _P, _P]),
+    "dk_extend_attention_kv4": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _I64, _I64, _I32,
+                                               ctypes.POINTER(_I32), ctypes.POINTER(_I32),
+                                               ctypes.POINTER(_I32), _P, _P, _SZ, _I32, _I64, _I32,
+                                               _I32, _I32, _I64, _I32,
+                                               ctypes.POINTER(DkExtendStrides), ctypes.c_float,
+                                               ctypes.c_float, _I32, _P, _P]),
     "dk_decode_partials": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _SZ, _I32, _I32, _I32, _I32,
                                           _I32, _I64, _I64, _I32, ctypes.POINTER(DkStrides),
                                           _I32, ctypes.POINTER(DkOptions), _P]),

@@ -431,6 +431,21 @@ int dk_extend_attention(const void* q, const void* k_pool, const void* v_pool,
                         float v_scale, float logit_cap, int32_t window, const float* sinks,
                         void* hip_stream);
 
+/* dk_extend_attention over a 4-bit cache (DK_KV_MXFP4; kv_p, kv_h in bytes): the K and V of request
+ * b's position p lie in page block_table[rows[b]][p / 16] (rows table_stride entries apart, num_rows
+ * of them, max_blocks entries each; a page id outside [0, num_pages) gives NaN to the tokens that
+ * attend to it). strides: q_b, q_h, o_b, o_h. The same workspace (dk_extend_workspace_bytes). In fp16,
+ * cache values beyond twice fp16's range become infinite. No counterpart in the reference. */
+int dk_extend_attention_kv4(const void* q, const void* cache, int64_t kv_p, int64_t kv_h,
+                            const int32_t* block_table, int64_t table_stride, int64_t num_rows,
+                            int32_t max_blocks, const int32_t* rows, const int32_t* new_lens,
+                            const int32_t* all_lens, void* out, void* workspace,
+                            size_t workspace_bytes, int32_t batch, int64_t num_tokens,
+                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                            int64_t num_pages, int32_t dtype, const dk_extend_strides* strides,
+                            float score_scale, float logit_cap, int32_t window,
+                            const float* sinks, void* hip_stream);
+
 /* Pass 1 only: writes partial_O / partial_m / partial_l for split_kv >= 1 splits into
  * the workspace (layout from dk_partials_layout; partial_m is the split's max of
  * q.k*scale, -1e9 for an empty split, partial_l = sum exp(score - partial_m),
