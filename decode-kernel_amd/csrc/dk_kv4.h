@@ -30,16 +30,19 @@ __device__ __forceinline__ int kv4_v_off(int d, int t, int i) {
 }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef u32 u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+typedef float f32x32v __attribute__((ext_vector_type(32)));
 
-// C += A.B: A 16 tokens x 128 dims of E2M1 (16 bytes per lane), B 128 dims x 16 columns of E4M3
-// (32 bytes per lane). sa / sb: E8M0 scales of the lane's row / column and 32-dim block (byte
-// GB of sb). The lanes' k index: fp4 lane r holds k = 32 r .. 32 r + 31; fp8 lane r holds k =
-// 16 r .. 16 r + 15 and 64 + 16 r .. 64 + 16 r + 15.
+// C += A.B: A 16 tokens x 128 dims of E2M1 (16 bytes per lane), B 128 dims x 16 columns of E2M3
+// (24 bytes per lane); lane row r holds k = 32 r .. 32 r + 31 of both. sa / sb: E8M0 scales of the
+// lane's row / column for those 32 (byte GB of sb). The products are multiples of 1/16 up to 45 (times
+// the scales), and the MFMA adds them exactly.
 template <int GB>
-__device__ __forceinline__ f32x4 mfma_mx(u32x4 a, i32x8 b, f32x4 c, u32 sa, u32 sb) {
+__device__ __forceinline__ f32x4 mfma_mx(u32x4 a, u32x6 b, f32x4 c, u32 sa, u32 sb) {
   const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, b, c, 4, 0, 0, (int)sa, GB, (int)sb);
+  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], (int)b[4], (int)b[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 2, 0, (int)sa, GB, (int)sb);
 }
 
 // bf16 pair (dims 2B, 2B+1 of the word's 8) of E2M1 codes times the scale whose exponent field
@@ -67,14 +70,13 @@ __device__ __forceinline__ u32 e8m0_exp(u32 w) {
   else return w << (23 - 8 * B);
 }
 
-// q enters the MX products as QParts parts of E4M3, each with a power-of-two scale per 32-dim
-// block. v_mfma_scale adds the products of a group of dims in a window of 13 bits below the
-// largest (measured: next to 2^8, 2^-5 counts and 2^-6 is lost). So the first part is a fixed-point
-// digit, whose products fill at most 8 bits and add up exactly: q to the nearest multiple of 1/16
-// of the power of two above the block's largest magnitude. The others are the remainder's leading 4
-// bits each time, with the sign of the next remainder 9 bits (bf16, 2 parts) or 13 (fp16, 3), so
-// that q's own 8 or 11 bits are held wherever it lies, and what the window drops is below 2^-18 of a
-// product of the largest magnitudes.
+// q enters the MX products as QParts parts of E2M3 (steps of 1/8 up to 2, 1/4 up to 4), each with a
+// power-of-two scale per 32-dim block: the first puts the block's largest magnitude in [2, 4), each
+// next one is 2^-5 of the last and holds what that left (at most 1/8 of its scale, so 4 of the next). 3
+// parts leave at most 2^-14 of the power of two below the block's largest magnitude, 4 parts 2^-19:
+// bf16's 8 bits are whole down to 2^-7 of the largest and fp16's 11 bits down to 2^-9, and what smaller
+// elements lose is no more than the largest one's own last bit. fp6 operands multiply at twice
+// the rate of fp8 ones, whose sums the MFMA also cuts 13 bits below a group's largest product.
 template <class T>
 struct QParts {
   static constexpr int n = 3;
@@ -84,33 +86,22 @@ struct QParts<F16> {
   static constexpr int n = 4;
 };
 // Part i's scale exponent below the block's largest exponent
-__device__ __forceinline__ constexpr int q_part_exp(int i) { return i == 0 ? 3 : 8 + 4 * i; }
-
-// Max over the lanes that hold one q head of HP (columns agreeing modulo HP)
-template <int HP>
-__device__ __forceinline__ float max_head(float x) {
-  if constexpr (HP <= 4) x = fmaxf(x, row_ror<4>(x));
-  if constexpr (HP <= 8) x = fmaxf(x, row_ror<8>(x));
-  return max_xor32(max_xor16(x));
-}
-template <int HP>
-__device__ __forceinline__ float sum_head(float x) {
-  if constexpr (HP <= 4) x += row_ror<4>(x);
-  if constexpr (HP <= 8) x += row_ror<8>(x);
-  return sum_xor32(sum_xor16(x));
-}
+__device__ __forceinline__ constexpr int q_part_exp(int i) { return 1 + 5 * i; }
 
 // One wavefront over pages of one kv head, kStep at a time, for up to HP (4, 8 or 16) q heads.
-//   * q.k: K's codes and scales are MFMA operands as they lie; q enters as E4M3 parts with
-//     scales of its own, one MFMA each. The 16 columns are HP heads x U = 16 / HP pages: for a
-//     page's MFMAs the scale of every other page's columns is 0 (2^-127), so U pages accumulate
-//     into one set of scores and every lane's 4 scores count: lane (r, c) holds tokens
-//     4r .. 4r+3 of page c / HP of the set, head c % HP.
+//   * q.k: K's codes and scales are MFMA operands as they lie; q enters as E2M3 parts with
+//     scales of its own, one MFMA each. The 16 columns are HP heads x U pages: for a page's MFMAs
+//     the scale of every other page's columns is 0 (2^-127), so U pages accumulate into one set of
+//     scores and every lane's 4 scores count: lane (r, c) holds tokens 4r .. 4r+3 of page group(c) of
+//     the set, head head(c).
 //   * softmax as in Wave: fp32, log2 domain, a reference that moves by more than 2^8 only.
 //   * P.V in bf16, whatever q's type: E2M1 times a power of two is exact there, and p as hi + lo
-//     parts keeps 16 bits at any magnitude. v_mfma_f32_16x16x32 over two pages: a lane's V words
-//     widened with their scales (v_cvt_scalef32_pk_bf16_fp4) and paired by token (v_perm). Rows
-//     are the heads again, so for HP < 16 hi and lo share one MFMA, lo in rows of its own.
+//     parts keeps 16 bits at any magnitude. A lane's V words are widened with their scales by
+//     v_cvt_scalef32_pk_bf16_fp4, two neighbouring dims of one token each, on v_mfma_f32_16x16x32.
+//     HP = 4: k = (token, parity): the pair is the operand as it is, and a row that is to sum the even
+//     dims has p in the even k and 0 in the odd ones. The 16 rows are 4 heads x (parity, part).
+//     HP = 8, 16: k = tokens of two pages, the pairs regrouped by token (v_perm); rows are the heads,
+//     and for HP = 8 the parts share an MFMA, each page's lo in the rows of the other page.
 template <class T, int D, int HP, bool CAP>
 struct Kv4Wave {
   static constexpr int kStep = D <= 128 ? 4 : 2;   // pages per step
@@ -122,19 +113,52 @@ struct Kv4Wave {
   static constexpr int W = D < 128 ? D : 128;
   static constexpr int JN = W / 16;                // dims per lane and part
   static constexpr int QP = QParts<T>::n;
+  static constexpr bool PAIR = HP == 4;            // P.V over (token, parity)
   static constexpr int ACC = HP == 16 ? 2 : 1;     // MFMAs per V operand (hi, lo)
+  static constexpr int OV = PAIR ? JN / 2 : JN;    // accumulators per part
+  static constexpr int kBatch = 64 / kStep;        // steps whose page offsets the lanes hold
 
-  i32x8 qf[NH][QP];
+  struct Pages {           // a step's pages as loaded
+    u32x4 k[kStep][NH], v[kStep][NH];
+    u32 ks[kStep][NH], vs[kStep][NH];
+  };
+  u32x6 qf[NH][QP];
   u32 qs[NH][QP];          // q's scales: byte g for the columns of page group g, 0 elsewhere
-  f32x4 o[NH][JN];         // row 4r + i (head (4r + i) % HP), dim 128 h + c * JN + j
+  f32x4 o[NH][OV];         // PAIR: head r, dims 2j + {0, 1, 0, 1} of the lane's run, parts hi, hi, lo,
+                           // lo; else row 4r + i (head (4r + i) % HP), dim 128 h + c * JN + j
   float mref, lsum;
-  u32x4 k[kStep][NH], v[kStep][NH];
-  u32 ks[kStep][NH], vs[kStep][NH];
   int r, c;
   u32 koff, voff, ksoff, vsoff;
   float kscale, cap_in, cap_out;
+  // the pages of a run: their ids from indices[idx0], n of them; steps w, w + NW, ...
+  const int32_t* ids;
+  const uint8_t* base;     // the kv head's block of page 0
+  uint64_t page_bytes;
+  uint32_t num_pages;
+  u32 off_lo, off_hi;      // lane l: byte offset of page l % kStep of step l / kStep of the batch
+  int32_t next_id;         // the next batch's page id
 
-  __device__ __forceinline__ void init(const Pass1Args& a) {
+  static __device__ __forceinline__ int head(int c) { return PAIR ? c >> 2 : c % HP; }
+  static __device__ __forceinline__ int group(int c) { return PAIR ? c & 3 : c / HP; }
+  // over the lanes that hold one q head
+  static __device__ __forceinline__ float max_head(float x) {
+    if constexpr (PAIR) {
+      x = fmaxf(x, xor1(x));
+      x = fmaxf(x, xor2(x));
+    }
+    if constexpr (HP == 8) x = fmaxf(x, row_ror<8>(x));
+    return max_xor32(max_xor16(x));
+  }
+  static __device__ __forceinline__ float sum_head(float x) {
+    if constexpr (PAIR) {
+      x += xor1(x);
+      x += xor2(x);
+    }
+    if constexpr (HP == 8) x += row_ror<8>(x);
+    return sum_xor32(sum_xor16(x));
+  }
+
+  __device__ __forceinline__ void init(const Pass1Args& a, int kvh) {
     const int lane = threadIdx.x & 63;
     r = lane >> 4;
     c = lane & 15;
@@ -145,87 +169,57 @@ struct Kv4Wave {
     kscale = a.kscale;
     cap_in = a.cap_in;
     cap_out = a.cap_out;
+    base = a.kv + (int64_t)kvh * a.kv_h;
+    page_bytes = (uint64_t)a.kv_p;
+    num_pages = a.num_pages;
   }
 
-  // q rows of the chunk's hv valid heads from qbase, q_h bytes apart, as E4M3 parts (QParts). A
+  // q rows of the chunk's hv valid heads from qbase, q_h bytes apart, as E2M3 parts (QParts). A
   // block with a NaN or an infinity gets the NaN scale.
   __device__ __forceinline__ void load_q(const uint8_t* qbase, int64_t q_h, int hv) {
-    const int h = c % HP;
+    const int h = head(c);
+    constexpr int NW_ = D == 64 ? 8 : 16;          // q words per lane and part
 #pragma unroll
     for (int p = 0; p < NH; ++p) {
-      // this lane's dims (see mfma_mx): 16 from d0 in bytes 0 .. 15, 16 from d1 in 16 .. 31; at
-      // D = 64 lane row r of K holds dims 16 r .. 16 r + 15 in the first half of its block
-      const int d0 = D == 64 ? 8 * r : 128 * p + 16 * r;
-      const int d1 = D == 64 ? 32 + 8 * r : d0 + 64;
-      const bool live = h < hv && (D != 64 || (r & 1) == 0);
-      float x[2][16];
-      u32 top[2];
+      // the dims that K's lane row r holds: 32 from 128 p + 32 r (D = 64: 16 from 16 r, and zeros)
+      u32 w[16];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        u32 w[8];
+      for (int i = 0; i < 16; ++i) w[i] = 0u;
+      if (h < hv) ld_words_cached<NW_>(w, qbase + (int64_t)h * q_h + 4 * NW_ * (4 * p + r));
+      f32x16v lo, hi;                              // even and odd dims
+      u32 top = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 0u;
-        if (live) ld_words_cached<8>(w, qbase + (int64_t)h * q_h + 2 * (e ? d1 : d0));
-        top[e] = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          unpack2(w[i], &x[e][2 * i], &x[e][2 * i + 1]);
-          top[e] = max(top[e], __builtin_bit_cast(u32, x[e][2 * i]) & 0x7fffffffu);
-          top[e] = max(top[e], __builtin_bit_cast(u32, x[e][2 * i + 1]) & 0x7fffffffu);
-        }
-        // a 32-dim block of q: lane rows 2 (r / 2) and 2 (r / 2) + 1 (D = 64: rows 0 and 2)
-        top[e] = max(top[e], (u32)__shfl_xor((int)top[e], D == 64 ? 32 : 16, 64));
-        if constexpr (D == 64) top[e] = max(top[e], (u32)__shfl_xor((int)top[e], 16, 64));
+      for (int i = 0; i < 16; ++i) {
+        float x, y;
+        unpack2(w[i], &x, &y);
+        lo[i] = x;
+        hi[i] = y;
+        top = max(top, __builtin_bit_cast(u32, x) & 0x7fffffffu);
+        top = max(top, __builtin_bit_cast(u32, y) & 0x7fffffffu);
       }
-      int ex[2];
+      if constexpr (D == 64) top = max(top, (u32)__shfl_xor((int)top, 16, 64));   // the other half
+      const int e = (int)(top >> 23);
+      const int ex = top == 0u ? 127 : max(e, q_part_exp(QP - 1) + 1);   // 255: NaN or infinity
+      static_for<QP>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const float sc = __builtin_bit_cast(float, (u32)(min(ex, 254) - q_part_exp(i)) << 23);
+        const u32x6 q6 = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(lo, hi, sc);
+        // the conversion writes its result before it has read all its inputs, which the compiler
+        // does not know: inputs that live on share no register with it (measured: a result over the
+        // scale's or a source's register was wrong)
+        asm volatile("" ::"v"(lo), "v"(hi), "v"(sc), "v"(q6));
+        qf[p][i] = q6;
+        qs[p][i] = (u32)(ex == 255 ? 255 : ex - q_part_exp(i)) << (8 * group(c));
+        if constexpr (i + 1 < QP) {
+          const f32x32v back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q6, sc);
+          asm volatile("" ::"v"(q6), "v"(sc), "v"(back));
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int b = (int)(top[e] >> 23);
-        ex[e] = top[e] == 0u ? 127 : max(b, q_part_exp(QP - 1) + 1);   // 255: NaN or infinity
-      }
-#pragma unroll
-      for (int i = 0; i < QP; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float sc = __builtin_bit_cast(float, (u32)(min(ex[e], 254) - q_part_exp(i)) << 23);
-          float y4[16];
-          if (i == 0) {                              // 1 / sc is a power of two too
-            const float inv = __builtin_bit_cast(
-                float, (u32)(254 - (min(ex[e], 254) - q_part_exp(0))) << 23);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) y4[y] = __builtin_rintf(x[e][y] * inv) * sc;
-          } else {
-#pragma unroll
-            for (int y = 0; y < 16; ++y) y4[y] = x[e][y];
-          }
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            i16x2 q8 = {0, 0};
-            q8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q8, y4[4 * y], y4[4 * y + 1], sc, false);
-            q8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q8, y4[4 * y + 2], y4[4 * y + 3], sc, true);
-            const u32 word = __builtin_bit_cast(u32, q8);
-            qf[p][i][4 * e + y] = (int)word;
-            const f32x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, sc, false);
-            const f32x2 a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, sc, true);
-            x[e][4 * y] -= a0[0];
-            x[e][4 * y + 1] -= a0[1];
-            x[e][4 * y + 2] -= a1[0];
-            x[e][4 * y + 3] -= a1[1];
+          for (int j = 0; j < 16; ++j) {
+            lo[j] -= back[2 * j];
+            hi[j] -= back[2 * j + 1];
           }
         }
-      }
-      // the scale of this lane's column and block r (D = 64: block r / 2): held by lane row
-      // 2 (r % 2) (D = 64: by every row), first half for r < 2
-      int e0 = ex[0], e1 = ex[1];
-      if constexpr (D != 64) {
-        const int src = ((r & 1) << 5) | c;
-        e0 = __shfl(ex[0], src, 64);
-        e1 = __shfl(ex[1], src, 64);
-      }
-      const int mine = r < 2 ? e0 : e1;
-#pragma unroll
-      for (int i = 0; i < QP; ++i)
-        qs[p][i] = (u32)(mine == 255 ? 255 : mine - q_part_exp(i)) << (8 * (c / HP));
+      });
     }
   }
 
@@ -244,51 +238,66 @@ struct Kv4Wave {
 #pragma unroll
     for (int p = 0; p < NH; ++p)
 #pragma unroll
-      for (int j = 0; j < JN; ++j) o[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < OV; ++j) o[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     mref = kMinit;
     lsum = 0.f;
   }
 
-  // loads of page slot I (a block that does not exist: a zero extent, zeros and no access)
+  // ---- pages
+  // This lane's page of the batch from step k0: id of page l % kStep of step k0 + l / kStep of the run
+  // (past its end: the last one's)
+  __device__ __forceinline__ int32_t lane_id(int NW, int w, int n, int k0) const {
+    const int lane = threadIdx.x & 63;
+    return ids[min(kStep * (w + NW * (k0 + lane / kStep)) + lane % kStep, n - 1)];
+  }
+  __device__ __forceinline__ void take_ids() {     // next_id becomes the batch's offsets
+    const uint64_t pid = (u32)next_id < num_pages ? (u32)next_id : 0u;
+    const uint64_t off = pid * page_bytes;
+    off_lo = (u32)off;
+    off_hi = (u32)(off >> 32);
+  }
+  // loads of page slot I from the lanes' offsets (live == false: a zero extent, zeros and no access)
   template <int I>
-  __device__ __forceinline__ void load_k(const uint8_t* blk, bool live) {
-    const __amdgpu_buffer_rsrc_t rs = page_rsrc(blk, live ? (u32)kv4_bytes(D) : 0u);
+  __device__ __forceinline__ void load(Pages& b, int lane, bool live) const {
+    const uint64_t off = (u32)__builtin_amdgcn_readlane((int)off_lo, lane) |
+                         (uint64_t)(u32)__builtin_amdgcn_readlane((int)off_hi, lane) << 32;
+    const __amdgpu_buffer_rsrc_t rs = page_rsrc(base + off, live ? (u32)kv4_bytes(D) : 0u);
     static_for<NH>([&](auto pc) {
       constexpr int p = decltype(pc)::value;
-      u32 w[4] = {0u, 0u, 0u, 0u};
+      u32 w[4] = {0u, 0u, 0u, 0u}, x[4] = {0u, 0u, 0u, 0u};
       ld_buf<KWD>(w, rs, koff, 64 * p);
-      k[I][p] = u32x4{w[0], w[1], w[2], w[3]};
-      ks[I][p] = (u32)__builtin_amdgcn_raw_buffer_load_b8(rs, (int)ksoff, 64 * p, kBufNT);
+      b.k[I][p] = u32x4{w[0], w[1], w[2], w[3]};
+      b.ks[I][p] = (u32)__builtin_amdgcn_raw_buffer_load_b8(rs, (int)ksoff, 64 * p, kBufNT);
+      ld_buf<VWD>(x, rs, voff, 1024 * p);
+      b.v[I][p] = u32x4{x[0], x[1], x[2], x[3]};
+      b.vs[I][p] = (u32)__builtin_amdgcn_raw_buffer_load_b32(rs, (int)vsoff, 64 * p, kBufNT);
     });
   }
-  template <int I>
-  __device__ __forceinline__ void load_v(const uint8_t* blk, bool live) {
-    const __amdgpu_buffer_rsrc_t rs = page_rsrc(blk, live ? (u32)kv4_bytes(D) : 0u);
-    static_for<NH>([&](auto pc) {
-      constexpr int p = decltype(pc)::value;
-      u32 w[4] = {0u, 0u, 0u, 0u};
-      ld_buf<VWD>(w, rs, voff, 1024 * p);
-      v[I][p] = u32x4{w[0], w[1], w[2], w[3]};
-      vs[I][p] = (u32)__builtin_amdgcn_raw_buffer_load_b32(rs, (int)vsoff, 64 * p, kBufNT);
+  // step k of this wavefront (its pages' offsets are in the lanes), which is global step w + NW * k
+  __device__ __forceinline__ void fetch(Pages& b, int NW, int w, int n, int k) const {
+    const int first = kStep * (w + NW * k), lane = kStep * (k % kBatch);
+    static_for<kStep>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      load<i>(b, lane + i, first + i < n);
     });
   }
 
-  // Tokens of page slot I outside [lo, hi): their scales may hold anything, so K's becomes 1 (a
-  // NaN would reach the scores of the set's other pages) and V's 0.
+  // Tokens of page slot I outside [lo, hi) of the page: their scales may hold anything, so K's becomes
+  // 1 (a NaN would reach the scores of the set's other pages) and V's 0.
   template <int I>
-  __device__ __forceinline__ void mask_scales(int lo, int hi) {
+  __device__ __forceinline__ void mask_scales(Pages& b, int lo, int hi) const {
     u32 m = 0u;
 #pragma unroll
     for (int t = 0; t < 4; ++t) m |= 4 * r + t >= lo && 4 * r + t < hi ? 0xffu << (8 * t) : 0u;
 #pragma unroll
     for (int p = 0; p < NH; ++p) {
-      ks[I][p] = c >= lo && c < hi ? ks[I][p] : 127u;
-      vs[I][p] &= m;
+      b.ks[I][p] = c >= lo && c < hi ? b.ks[I][p] : 127u;
+      b.vs[I][p] &= m;
     }
   }
 
   // Scores of the step's pages
-  __device__ __forceinline__ void scores(f32x4 (&s)[SETS]) {
+  __device__ __forceinline__ void scores(const Pages& b, f32x4 (&s)[SETS]) const {
     static_for<SETS>([&](auto xc) {
       constexpr int x = decltype(xc)::value;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -298,54 +307,57 @@ struct Kv4Wave {
         for (int p = 0; p < NH; ++p)
 #pragma unroll
           for (int i = 0; i < QP; ++i)
-            acc = mfma_mx<g>(k[x * U + g][p], qf[p][i], acc, ks[x * U + g][p], qs[p][i]);
+            acc = mfma_mx<g>(b.k[x * U + g][p], qf[p][i], acc, b.ks[x * U + g][p], qs[p][i]);
       });
       s[x] = acc;
     });
   }
 
-  // The running softmax over the step's scores: s becomes p. valid: of page slot i in 16 bits
-  // from bit 16 i.
-  __device__ __forceinline__ void softmax(f32x4 (&s)[SETS], bool edge, uint64_t valid) {
+  // The running softmax over the step's scores: s becomes p. edge: the step's tokens outside
+  // [lo, hi) (from the step's first) do not count.
+  __device__ __forceinline__ void softmax(f32x4 (&s)[SETS], bool edge, int lo, int hi) {
     float mx = kNegInf;
 #pragma unroll
     for (int x = 0; x < SETS; ++x) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[x][i] = CAP ? cap_out * tanh_approx(s[x][i] * cap_in) : s[x][i] * kscale;
+        if constexpr (U * HP < 16) s[x][i] = group(c) < U ? s[x][i] : kNegInf;   // no such page
       }
-    }
-    if constexpr (U * HP < 16) {                   // columns without a page
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[0][i] = c < U * HP ? s[0][i] : kNegInf;
     }
     if (edge) {
 #pragma unroll
-      for (int x = 0; x < SETS; ++x) {
-        const int vl = (int)(valid >> (16 * (x * U + c / HP % U)));   // this lane's page
-        const int lo = vl >> 8 & 255, hi = vl & 255;
+      for (int x = 0; x < SETS; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[x][i] = 4 * r + i >= lo && 4 * r + i < hi && (U * HP == 16 || c < U * HP) ? s[x][i]
-                                                                                     : kNegInf;
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int t = kPage * (x * U + group(c)) + 4 * r + i;
+          s[x][i] = t >= lo && t < hi ? s[x][i] : kNegInf;
+        }
     }
 #pragma unroll
     for (int x = 0; x < SETS; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[x][i]);
     if (__builtin_amdgcn_ballot_w64(mx > mref + kSlack)) {
-      const float mn = fmaxf(mref, max_head<HP>(mx));
+      const float mn = fmaxf(mref, max_head(mx));
       const float al = __builtin_amdgcn_exp2f(mref - mn);
       lsum *= al;
       mref = mn;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {                // row 4r + i's head is column (4r + i) % HP's
-        const float f = __shfl(al, (4 * r + i) % HP, 16);
+      if constexpr (PAIR) {                          // the accumulators are head r's
+        const float f = __shfl(al, 4 * r, 16);
 #pragma unroll
         for (int p = 0; p < NH; ++p)
 #pragma unroll
-          for (int j = 0; j < JN; ++j) o[p][j][i] *= f;
+          for (int j = 0; j < OV; ++j) o[p][j] *= f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = __shfl(al, (4 * r + i) % HP, 16);
+#pragma unroll
+          for (int p = 0; p < NH; ++p)
+#pragma unroll
+            for (int j = 0; j < OV; ++j) o[p][j][i] *= f;
+        }
       }
     }
 #pragma unroll
@@ -356,10 +368,42 @@ struct Kv4Wave {
     }
   }
 
-  // The A operands of P.V: pair m holds pages 2m (words 0, 1) and 2m + 1 (words 2, 3), rows =
-  // columns of the scores. HP = 16: hi in pa[m][0], lo in pa[m][1]. HP = 8: rows of group g hold
-  // page 2m + g's hi and the other page's lo. HP = 4: page i's hi in rows of group i, its lo in
-  // rows of group i ^ 2, zero in the other pages' rows.
+  // ---- P.V over (token, parity)
+  __device__ __forceinline__ void accumulate_pair(const Pages& b, const f32x4 (&s)[SETS]) {
+    // a token's p as (hi, lo) in one word: hi rounded to the nearest, lo the remainder cut to bf16
+    u32 t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = s[0][i];
+      const u32 h = (__builtin_bit_cast(u32, x) + 0x8000u) & 0xffff0000u;
+      const float l = x - __builtin_bit_cast(float, h);
+      t[i] = __builtin_amdgcn_perm(__builtin_bit_cast(u32, l), h, 0x07060302u);
+    }
+    // row 4 head + x: parity x & 1, part x >> 1: this lane's part of the word to its parity's half
+    const u32 sel = (c & 1) ? ((c & 2) ? 0x03020c0cu : 0x01000c0cu) : ((c & 2) ? 0x0c0c0302u : 0x0c0c0100u);
+    static_for<kStep>([&](auto uc) {
+      constexpr int u = decltype(uc)::value;
+      u32x4 pa;                                      // page u's weights lie in lane u of each quad
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32 y = quad_bcast_u<u>(t[i]);
+        pa[i] = __builtin_amdgcn_perm(y, y, sel);
+      }
+#pragma unroll
+      for (int p = 0; p < NH; ++p)
+        static_for<OV>([&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          u32 v[4];
+          widen<j>(b, u, p, v);
+          o[p][j] = BF16::mfma(pa, u32x4{v[0], v[1], v[2], v[3]}, o[p][j]);
+        });
+    });
+  }
+
+  // ---- P.V over the tokens of two pages
+  // The A operands: pair m holds pages 2m (words 0, 1) and 2m + 1 (words 2, 3), rows = columns of
+  // the scores. HP = 16: hi in pa[m][0], lo in pa[m][1]. HP = 8: rows of group g hold page 2m + g's
+  // hi and the other page's lo.
   __device__ __forceinline__ void weights(const f32x4 (&s)[SETS], u32x4 (&pa)[kStep / 2][ACC]) const {
     u32 hi[SETS][2], lo[SETS][2];
 #pragma unroll
@@ -378,141 +422,137 @@ struct Kv4Wave {
       }
     } else {
 #pragma unroll
-      for (int x = 0; x < SETS; ++x)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) lo[x][e] = dpp_u<0x128>(lo[x][e]);   // from column c ^ 8
-      if constexpr (HP == 8) {
-#pragma unroll
-        for (int m = 0; m < SETS; ++m)
-          pa[m][0] = u32x4{c < 8 ? hi[m][0] : lo[m][0], c < 8 ? hi[m][1] : lo[m][1],
-                           c < 8 ? lo[m][0] : hi[m][0], c < 8 ? lo[m][1] : hi[m][1]};
-      } else {
-        const u32 even = (c >> 2 & 1) ? 0u : ~0u, own = c < 8 ? ~0u : 0u;
-        const u32 d0 = hi[0][0] ^ lo[0][0], d1 = hi[0][1] ^ lo[0][1];
-        static_for<kStep / 2>([&](auto mc) {         // pages 0, 1 then 2, 3
-          constexpr int m = decltype(mc)::value;
-          const u32 pick = m == 0 ? own : ~own;      // hi there, lo elsewhere
-          const u32 x0 = lo[0][0] ^ (d0 & pick), x1 = lo[0][1] ^ (d1 & pick);
-          pa[m][0] = u32x4{x0 & even, x1 & even, x0 & ~even, x1 & ~even};
-        });
+      for (int m = 0; m < SETS; ++m) {
+        const u32 l0 = dpp_u<0x128>(lo[m][0]), l1 = dpp_u<0x128>(lo[m][1]);   // from column c ^ 8
+        pa[m][0] = u32x4{c < 8 ? hi[m][0] : l0, c < 8 ? hi[m][1] : l1, c < 8 ? l0 : hi[m][0],
+                         c < 8 ? l1 : hi[m][1]};
       }
     }
   }
-
-  // dims 2b, 2b+1 of this lane's run (part p) for its 4 tokens of page slot i: words (tokens
-  // 0, 1) and (2, 3) of the even dim in e, of the odd dim in d
-  template <int B>
-  __device__ __forceinline__ void widen(int i, int p, u32 (&e)[2], u32 (&d)[2]) const {
-    u32 t[4];
-    static_for<4>([&](auto tc) {
-      constexpr int x = decltype(tc)::value;
-      const u32 sc = e8m0_exp<x>(vs[i][p]);
-      if constexpr (D == 64) t[x] = fp4_bf16<2 * (x % 2) + B>(v[i][p][x / 2], sc);
-      else t[x] = fp4_bf16<B>(v[i][p][x], sc);
-    });
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      e[x] = __builtin_amdgcn_perm(t[2 * x + 1], t[2 * x], 0x05040100u);
-      d[x] = __builtin_amdgcn_perm(t[2 * x + 1], t[2 * x], 0x07060302u);
-    }
-  }
-
-  __device__ __forceinline__ void accumulate(const u32x4 (&pa)[kStep / 2][ACC]) {
+  __device__ __forceinline__ void accumulate_tokens(const Pages& b, const f32x4 (&s)[SETS]) {
+    u32x4 pa[kStep / 2][ACC];
+    weights(s, pa);
     static_for<kStep / 2>([&](auto mc) {
       constexpr int m = decltype(mc)::value;
 #pragma unroll
       for (int p = 0; p < NH; ++p)
         static_for<JN / 2>([&](auto bc) {
-          constexpr int b = decltype(bc)::value;
-          u32 e0[2], d0[2], e1[2], d1[2];
-          widen<b>(2 * m, p, e0, d0);
-          widen<b>(2 * m + 1, p, e1, d1);
-          const u32x4 ve = {e0[0], e0[1], e1[0], e1[1]}, vd = {d0[0], d0[1], d1[0], d1[1]};
+          constexpr int j = decltype(bc)::value;
+          u32 x[4], y[4];
+          widen<j>(b, 2 * m, p, x);
+          widen<j>(b, 2 * m + 1, p, y);
+          const u32x4 ve = {pair_lo(x[0], x[1]), pair_lo(x[2], x[3]), pair_lo(y[0], y[1]), pair_lo(y[2], y[3])};
+          const u32x4 vd = {pair_hi(x[0], x[1]), pair_hi(x[2], x[3]), pair_hi(y[0], y[1]), pair_hi(y[2], y[3])};
 #pragma unroll
-          for (int x = 0; x < ACC; ++x) {
-            o[p][2 * b] = BF16::mfma(pa[m][x], ve, o[p][2 * b]);
-            o[p][2 * b + 1] = BF16::mfma(pa[m][x], vd, o[p][2 * b + 1]);
+          for (int e = 0; e < ACC; ++e) {
+            o[p][2 * j] = BF16::mfma(pa[m][e], ve, o[p][2 * j]);
+            o[p][2 * j + 1] = BF16::mfma(pa[m][e], vd, o[p][2 * j + 1]);
           }
         });
     });
   }
+  static __device__ __forceinline__ u32 pair_lo(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+  static __device__ __forceinline__ u32 pair_hi(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-  // Pages 0 .. n-1 of a run, groups of kStep first + w, + NW, ...; block(i): the page block of
-  // page i; valid(i): its tokens, hi | lo << 8. K's next loads are issued when the scores have
-  // read the registers, V's when P.V has: the other half of a step covers each.
-  template <class BlockFn, class ValidFn>
-  __device__ __forceinline__ void stream(int NW, int w, int n, BlockFn block, ValidFn valid) {
-    const int groups = (n + kStep - 1) / kStep;
-    if (w >= groups) return;
-    const uint8_t* at[kStep];
-    static_for<kStep>([&](auto ic) {
-      constexpr int i = decltype(ic)::value;
-      at[i] = block(min(kStep * w + i, n - 1));
-      load_k<i>(at[i], kStep * w + i < n);
+  // dims 2J, 2J+1 of this lane's run (part p) for its 4 tokens of page slot i, as bf16 pairs
+  template <int J>
+  static __device__ __forceinline__ void widen(const Pages& b, int i, int p, u32 (&t)[4]) {
+    static_for<4>([&](auto tc) {
+      constexpr int x = decltype(tc)::value;
+      const u32 sc = e8m0_exp<x>(b.vs[i][p]);
+      if constexpr (D == 64) t[x] = fp4_bf16<2 * (x % 2) + J>(b.v[i][p][x / 2], sc);
+      else t[x] = fp4_bf16<J>(b.v[i][p][x], sc);
     });
-    static_for<kStep>([&](auto ic) {
-      constexpr int i = decltype(ic)::value;
-      load_v<i>(at[i], kStep * w + i < n);
-    });
-    for (int g = w; g < groups; g += NW) {
-      const int next = g + NW;
-      uint64_t vl = 0;
+  }
+
+  // One loaded step, its pages from page `first` of the run; tokens [lo, hi) of the run count
+  __device__ __forceinline__ void compute(Pages& b, int first, int lo, int hi) {
+    lo -= kPage * first;
+    hi -= kPage * first;
+    const bool edge = lo > 0 || hi < kStep * kPage;
+    if (edge) {
       static_for<kStep>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        vl |= (uint64_t)(kStep * g + i < n ? valid(kStep * g + i) : 0) << (16 * i);
-        at[i] = block(min(kStep * next + i, n - 1));
+        mask_scales<i>(b, lo - kPage * i, hi - kPage * i);
       });
-      const bool edge = vl != (kStep == 4 ? 0x0010001000100010u : 0x00100010u);
-      if (edge) {
-        static_for<kStep>([&](auto ic) {
-          constexpr int i = decltype(ic)::value;
-          mask_scales<i>((int)(vl >> (16 * i + 8)) & 255, (int)(vl >> (16 * i)) & 255);
-        });
+    }
+    f32x4 s[SETS];
+    scores(b, s);
+    softmax(s, edge, lo, hi);
+    if constexpr (PAIR) accumulate_pair(b, s);
+    else accumulate_tokens(b, s);
+  }
+
+  // The run's first loads: the ids of the first batch of steps of pages indices[0 .. n)
+  __device__ __forceinline__ void start(const int32_t* indices, int NW, int w, int n, Pages& b) {
+    ids = indices;
+    next_id = lane_id(NW, w, n, 0);
+    take_ids();
+    fetch(b, NW, w, n, 0);
+  }
+  // Steps of a run of n pages after start(), whose n may have been larger; tokens [lo, hi) count. The
+  // next step's loads are in flight while one is computed.
+  __device__ __forceinline__ void stream(int NW, int w, int n, int lo, int hi, Pages& b0) {
+    const int all = (n + kStep - 1) / kStep;
+    const int steps = all > w ? (all - w + NW - 1) / NW : 0;
+    if (steps == 0) return;
+    if (steps > kBatch - 1) next_id = lane_id(NW, w, n, kBatch);
+    Pages b1;
+    auto step = [&](Pages& cur, Pages& nxt, int k) {
+      const int kn = k + 1;
+      if (kn % kBatch == 0) {                        // the lanes' batch of offsets is used up
+        take_ids();
+        next_id = lane_id(NW, w, n, kn + kBatch);
       }
-      f32x4 s[SETS];
-      scores(s);
-      static_for<kStep>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        load_k<i>(at[i], kStep * next + i < n);
-      });
-      softmax(s, edge, vl);
-      u32x4 pa[kStep / 2][ACC];
-      weights(s, pa);
-      accumulate(pa);
-      static_for<kStep>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        load_v<i>(at[i], kStep * next + i < n);
-      });
+      fetch(nxt, NW, w, n, kn);
+      compute(cur, kStep * (w + NW * k), lo, hi);
+    };
+    for (int k = 0;;) {
+      step(b0, b1, k);
+      if (++k >= steps) break;
+      step(b1, b0, k);
+      if (++k >= steps) break;
     }
   }
 };
 
-// LDS for the wavefronts' results: o's 16 rows, references and sums per head
-template <int D, int NW>
+// LDS for the wavefronts' results: the accumulators' rows, references and sums per head
+template <int D, int HP, int NW>
 struct Kv4Smem {
-  alignas(16) float o[NW][16][D];
+  static constexpr int ROWS = HP == 4 ? 4 : 16;
+  alignas(16) float o[NW][ROWS][D];
   float m[NW][16], l[NW][16];
 };
 
 // The workgroup's result for hv heads: normalised to out, or a partial (head h at row
 // prow0 + h * phstride). Holds workgroup barriers.
 template <class T, int D, int HP, int NW, class WV>
-__device__ __forceinline__ void kv4_store(WV& wv, Kv4Smem<D, NW>& sm, const Pass1Args& a,
+__device__ __forceinline__ void kv4_store(WV& wv, Kv4Smem<D, HP, NW>& sm, const Pass1Args& a,
                                           bool direct, uint8_t* out, int64_t prow0,
                                           int64_t phstride, int hv, int w, int tid, int qh0) {
-  const float l = sum_head<HP>(wv.lsum);
-  if (wv.r == 0 && wv.c < HP) {
-    sm.m[w][wv.c] = wv.mref;
-    sm.l[w][wv.c] = l;
+  const float l = WV::sum_head(wv.lsum);
+  if (wv.r == 0 && WV::group(wv.c) == 0) {
+    sm.m[w][WV::head(wv.c)] = wv.mref;
+    sm.l[w][WV::head(wv.c)] = l;
   }
 #pragma unroll
-  for (int p = 0; p < WV::NH; ++p)
+  for (int p = 0; p < WV::NH; ++p) {
+    if constexpr (WV::PAIR) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < WV::OV; j += 2) {
+        const f32x4 x = wv.o[p][j], y = wv.o[p][j + 1];
+        *reinterpret_cast<f32x4*>(&sm.o[w][wv.r][128 * p + wv.c * WV::JN + 2 * j]) =
+            f32x4{x[0] + x[2], x[1] + x[3], y[0] + y[2], y[1] + y[3]};
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < WV::JN; j += 4)
-        *reinterpret_cast<f32x4*>(&sm.o[w][4 * wv.r + i][128 * p + wv.c * WV::JN + j]) =
-            f32x4{wv.o[p][j][i], wv.o[p][j + 1][i], wv.o[p][j + 2][i], wv.o[p][j + 3][i]};
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < WV::JN; j += 4)
+          *reinterpret_cast<f32x4*>(&sm.o[w][4 * wv.r + i][128 * p + wv.c * WV::JN + j]) =
+              f32x4{wv.o[p][j][i], wv.o[p][j + 1][i], wv.o[p][j + 2][i], wv.o[p][j + 3][i]};
+    }
+  }
   __syncthreads();
   const float* sink = a.sinks ? a.sinks + qh0 : nullptr;
   const bool out8 = (((uintptr_t)out | (uintptr_t)a.o_h) & 7) == 0;
@@ -528,8 +568,7 @@ __device__ __forceinline__ void kv4_store(WV& wv, Kv4Smem<D, NW>& sm, const Pass
       const float f = __builtin_amdgcn_exp2f(sm.m[ww][h] - mt);
       L += sm.l[ww][h] * f;
       f32x4 x = *reinterpret_cast<const f32x4*>(&sm.o[ww][h][d]);
-#pragma unroll
-      for (int g = 1; g < 16 / HP; ++g) x += *reinterpret_cast<const f32x4*>(&sm.o[ww][g * HP + h][d]);
+      if constexpr (HP == 8) x += *reinterpret_cast<const f32x4*>(&sm.o[ww][8 + h][d]);
       O += x * f;
     }
     const bool empty = !(mt > kMinit) && L == 0.f;
@@ -559,12 +598,16 @@ __device__ __forceinline__ void kv4_store(WV& wv, Kv4Smem<D, NW>& sm, const Pass
   __syncthreads();   // the LDS is reused by the next segment
 }
 
+// Wavefronts per SIMD that the kernels are compiled for: two, but for D = 256 with 8 or 16 heads, whose
+// accumulators and pages need more than 256 registers
+template <int D, int HP>
+constexpr int kv4_waves() { return D == 256 && HP > 4 ? 1 : 2; }
+
 // Explicit split: workgroup = (head chunk, kv head, split, sequence), as dk_pass1_split
 template <class T, int D, int HP, bool CAP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void dk_kv4_split(Pass1Args a) {
-  __shared__ Kv4Smem<D, NW> sm;
-  Kv4Wave<T, D, HP, CAP> wv;
-  wv.init(a);
+__global__ __launch_bounds__(NW * 64, (kv4_waves<D, HP>())) void dk_kv4_split(Pass1Args a) {
+  using WV = Kv4Wave<T, D, HP, CAP>;
+  __shared__ Kv4Smem<D, HP, NW> sm;
   const int w = uniform(threadIdx.x >> 6);
   int hc = 0, t = blockIdx.x;
   if (a.chunks > 1) {
@@ -576,6 +619,8 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_split(Pass1Args a) {
   const int kvh = t % a.hkv;
   t /= a.hkv;
   const int s = t % a.split, b = t / a.split;
+  WV wv;
+  wv.init(a, kvh);
   const int seq0 = seq_begin(a, b);
   const int npages = max(seq_begin(a, b + 1), seq0) - seq0;
   const int last = min(max(ld_const(a.last_len, b), 0), kPage);
@@ -591,32 +636,44 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_split(Pass1Args a) {
   const int n = max(min(p0 + pps, npages) - p0, 0);
   const int qh0 = kvh * a.group + hc * a.per;
   const int hv = min(a.per, a.group - hc * a.per);
+  typename WV::Pages pages;
+  if (n > 0) wv.start(a.indices + seq0 + p0, NW, w, n, pages);
   wv.load_q(a.q + (int64_t)b * a.q_b + (int64_t)qh0 * a.q_h, a.q_h, hv);
   wv.reset();
-  const uint8_t* base = a.kv + (int64_t)kvh * a.kv_h;
-  auto block = [&](int i) -> const uint8_t* {
-    u32 pid = (u32)uniform(ld_const(a.indices, seq0 + p0 + i));
-    pid = pid < a.num_pages ? pid : 0u;
-    return base + (int64_t)pid * a.kv_p;
-  };
-  auto valid = [&](int i) -> int {
-    const int pg = p0 + i;
-    return (pg == npages - 1 ? last : kPage) | (pg == first_page ? first_tok << 8 : 0);
-  };
-  wv.stream(NW, w, n, block, valid);
+  const int lo = p0 == first_page ? first_tok : 0;
+  const int hi = p0 + n == npages ? kPage * (n - 1) + last : kPage * n;
+  wv.stream(NW, w, n, lo, hi, pages);
   kv4_store<T, D, HP, NW>(wv, sm, a, a.direct != 0,
                           a.out + (int64_t)b * a.o_b + (int64_t)qh0 * a.o_h,
                           ((int64_t)b * a.hq + qh0) * a.split + s, a.split, hv, w,
                           (int)threadIdx.x, qh0);
 }
 
+// The sequence that holds unit u of the linear (sequence, page) space: the largest b with
+// start(b) <= u, by one wavefront's search over kv_indptr, 64 candidates per step (one dependent
+// read up to 64 sequences, two up to 4096); every lane returns it.
+__device__ __forceinline__ int kv4_sequence_of(const Pass1Args& a, int base, int u) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, S = a.batch;
+  while (S > 1) {
+    const int st = (S + 63) / 64;
+    const bool in = lane * st < S;
+    const int at = min(max(a.indptr[min(lo + lane * st, a.batch)], 0), a.num_indices) - base;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in && at <= u);
+    const int k = m ? 63 - __builtin_clzll(m) : 0;
+    lo += k * st;
+    S = min(st, S - k * st);
+  }
+  return uniform(lo);
+}
+
 // Balanced: the page ranges, segments and partial slots of dk_pass1_balanced (one kv head per
-// workgroup; the range split that charges sequence starts when a.seg_cost > 0)
+// workgroup; the range split that charges sequence starts when a.seg_cost > 0). A range's first pages
+// are on their way while its first sequence is looked up.
 template <class T, int D, int HP, bool CAP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void dk_kv4_balanced(Pass1Args a, int heads) {
-  __shared__ Kv4Smem<D, NW> sm;
-  Kv4Wave<T, D, HP, CAP> wv;
-  wv.init(a);
+__global__ __launch_bounds__(NW * 64, (kv4_waves<D, HP>())) void dk_kv4_balanced(Pass1Args a, int heads) {
+  using WV = Kv4Wave<T, D, HP, CAP>;
+  __shared__ Kv4Smem<D, HP, NW> sm;
   const int w = uniform(threadIdx.x >> 6);
   const int Wg = a.ranges;
   int hc, j;
@@ -630,6 +687,9 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_balanced(Pass1Args a, int h
     hc = (int)blockIdx.x % a.hkv;
     j = (int)blockIdx.x / a.hkv;
   }
+  const int kvh = hc % a.hkv, chunk = hc / a.hkv;
+  WV wv;
+  wv.init(a, kvh);
   const int base = seq_begin(a, 0);
   const int P = max(seq_begin(a, a.batch) - base, 0);
   const int A = a.seg_cost;
@@ -649,18 +709,11 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_balanced(Pass1Args a, int h
                 ? P : cost_boundary(a, base, P, A, (int64_t)(j + 1) * Lc, &b_end);
   }
   if (u >= u_end) return;
-  const int kvh = hc % a.hkv, chunk = hc / a.hkv;
   const int qh0 = kvh * a.group + chunk * a.per;
   const int hv = min(a.per, a.group - chunk * a.per);
-  const uint8_t* kbase = a.kv + (int64_t)kvh * a.kv_h;
-  if (A == 0) {
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (seq_begin(a, mid) - base <= u) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-  }
+  typename WV::Pages pages;
+  wv.start(a.indices + base + u, NW, w, u_end - u, pages);
+  if (A == 0) b = kv4_sequence_of(a, base, u);
   int seq0 = seq_begin(a, b);
   int np = max(seq_begin(a, b + 1), seq0) - seq0;
   int pg = u - (seq0 - base);
@@ -676,16 +729,10 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_balanced(Pass1Args a, int h
     wv.load_q(a.q + (int64_t)b * a.q_b + (int64_t)qh0 * a.q_h, a.q_h, hv);
     wv.reset();
     const int last = min(max(ld_const(a.last_len, b), 0), kPage);
-    const int idx0 = seq0 + pg, left = np - 1 - pg;
-    auto block = [&](int i) -> const uint8_t* {
-      u32 pid = (u32)uniform(ld_const(a.indices, idx0 + i));
-      pid = pid < a.num_pages ? pid : 0u;
-      return kbase + (int64_t)pid * a.kv_p;
-    };
-    auto valid = [&](int i) -> int { return i == left ? last : kPage; };
-    wv.stream(NW, w, n, block, valid);
+    const int hi = pg + n == np ? kPage * (n - 1) + last : kPage * n;
+    wv.stream(NW, w, n, 0, hi, pages);
     // ranges holding this sequence's units
-    const int start = seq0 - base;
+    const int start = seq0 - base, cur = b;
     int nslots;
     if (A == 0) {
       nslots = (start + np - 1) / L - start / L + 1;
@@ -693,19 +740,23 @@ __global__ __launch_bounds__(NW * 64, 2) void dk_kv4_balanced(Pass1Args a, int h
       const int64_t c0 = (int64_t)start + (int64_t)A * b;
       nslots = (int)((c0 + np - 1) / Lc - c0 / Lc + 1);
     }
-    kv4_store<T, D, HP, NW>(wv, sm, a, nslots == 1,
-                            a.out + (int64_t)b * a.o_b + (int64_t)qh0 * a.o_h,
-                            ((int64_t)hc * (Wg + a.batch) + j + b) * heads, 1, hv, w,
-                            (int)threadIdx.x, qh0);
     u += n;
-    if (u >= u_end) break;
-    do {
-      ++b;
-      seq0 = seq_begin(a, b);
-      np = max(seq_begin(a, b + 1), seq0) - seq0;
-    } while (np == 0 && b < a.batch - 1);
-    if (np <= 0) break;                        // only for an invalid kv_indptr
-    pg = 0;
+    bool more = u < u_end;
+    if (more) {                                // the next sequence's first pages
+      do {
+        ++b;
+        seq0 = seq_begin(a, b);
+        np = max(seq_begin(a, b + 1), seq0) - seq0;
+      } while (np == 0 && b < a.batch - 1);
+      more = np > 0;                           // else only for an invalid kv_indptr
+      pg = 0;
+    }
+    kv4_store<T, D, HP, NW>(wv, sm, a, nslots == 1,
+                            a.out + (int64_t)cur * a.o_b + (int64_t)qh0 * a.o_h,
+                            ((int64_t)hc * (Wg + a.batch) + j + cur) * heads, 1, hv, w,
+                            (int)threadIdx.x, qh0);
+    if (!more) break;
+    wv.start(a.indices + seq0, NW, w, min(np, u_end - u), pages);
   }
 }
 
