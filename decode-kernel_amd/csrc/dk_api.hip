@@ -394,22 +394,39 @@ bool short_split_runs(const Problem& p, const Plan& pl, int cus) {
 }
 
 // ---- the 4-bit cache
-// Explicit split that split_kv == 0 runs (1: one pass), or 0 for the balanced schedule.
+// Explicit split that split_kv == 0 runs (1: one pass), or 0 for the balanced schedule. Four
+// wavefronts that keep two steps of pages in flight reach the read rate on a CU, so what decides
+// is the fixed cost (a merge is 3 to 4 us) and how evenly the workgroups fill the CUs; us per
+// replayed call, heads and head_dim 32/8/128 unless given:
+//  - up to kKv4OnePassPages pages (all that the hint or the window allows): one pass. 2 x 512
+//    tokens 6.3 against 9.2 balanced, 256 x 700 40.4 against 44.0.
+//  - near-uniform lengths (no sequence 5/4 of the mean, by the hint): parts that fill one workgroup
+//    per CU to 7/8 (D = 64, bound by instructions: two), none under a step of pages per wavefront.
+//    32 x 8192 tokens 49.5 in one pass, 50.8 in two parts, 52.9 balanced; 4 x 32768 (64/8) 29.7 in
+//    8 parts, 31.0; 8 x 4096 13.1 in 4, 14.2; 1 x 4096 8.1 in 16, 11.0; 1 x 131071 (128/8) 31.9 in
+//    32, 34.5; 32 x 8192 at D = 64 31.8 in 2, 34.2 in one pass, 32.9.
+//  - other lengths: balanced. 100 requests of 100 to 6000 tokens 64.2 against 70.5 in one pass.
 int kv4_auto_split(const Problem& p, const Plan& pl, int cus) {
+  const bool windowed = p.opt.window > 0;
+  if (!windowed && p.opt.schedule != 0) return p.opt.schedule == 2;
   const int64_t pairs = (int64_t)p.batch * pl.pairs_per_seq;
-  const int64_t groups = (int64_t)cus * kKv4WavesPerCU / kKv4Waves;
   const int64_t hint = p.opt.max_pages_per_seq;
-  int64_t s = 0;
-  if (p.opt.window > 0) {
-    const int64_t avg = p.num_indices / p.batch;
-    const int64_t pages = std::min<int64_t>(avg, p.opt.window / kPageSize + 2);
-    s = std::min(groups / pairs, pages / (2 * kKv4StepPages));
-    s = std::min<int64_t>(std::max<int64_t>(s, 1), kMaxSplit);
-  } else if (p.opt.schedule == 2) {
-    s = 1;
-  } else if (p.opt.schedule == 0 && hint > 0) {
-    const int64_t per = std::max<int64_t>(groups / pl.pairs_per_seq, 1);
-    if (pairs <= groups && hint <= (p.num_indices + per - 1) / per) s = 1;
+  int64_t pages = hint > 0 ? hint : p.batch == 1 || windowed ? p.num_indices / p.batch : 0;
+  if (windowed) pages = std::min<int64_t>(pages, p.opt.window / kPageSize + 2);
+  if (pages <= 0) return windowed;
+  if (pages <= kKv4OnePassPages) return 1;
+  if (!windowed && hint * p.batch * 4 > p.num_indices * 5) return 0;
+  const int64_t per_split = kKv4Waves * kKv4StepPages;
+  int64_t s = windowed;
+  for (int64_t groups : {(int64_t)cus, (int64_t)cus * 2}) {
+    if (p.head_dim == 64 && groups == cus && pairs <= cus) continue;
+    const int64_t rounds = (pairs + groups - 1) / groups;
+    const int64_t fill = std::max<int64_t>(groups / pairs, 1);
+    const int64_t most = std::max<int64_t>(pages / per_split, 1);
+    if (fill >= most || pairs * fill * 8 >= rounds * groups * 7) {
+      s = std::min<int64_t>(std::min(fill, most), kMaxSplit);
+      break;
+    }
   }
   for (; s > 1; --s) {
     size_t o, m, l, total;

@@ -156,6 +156,7 @@ constexpr int kGroupedAlwaysRowBytes = 64;
 constexpr int kKv4Waves = 4;
 constexpr int kKv4WavesPerCU = 8;
 constexpr int kKv4StepPages = 4;     // pages that a wavefront takes at a time (2 at D = 256)
+constexpr int kKv4OnePassPages = 64;  // longest sequence that one pass reads however few there are
 
 // Everything a launch needs that is known on the host.
 struct Problem {
