@@ -1,6 +1,6 @@
-// dk_native.cpp — decode_attention's call path as a CPython extension (module _dk_native):
-// reads the tensors' sizes, strides and types through ATen, checks them, allocates the output
-// and calls the C ABI. One call costs about as much as its launches; the same checks and
+// dk_native.cpp — decode_attention's call path as a CPython extension (module _dk_native), and
+// paging's of a 4-bit cache's step: reads the tensors' sizes, strides and types through ATen,
+// checks them, allocates the output and calls the C ABI. One call costs about as much as its launches; the same checks and
 // argument marshalling in Python cost 8-10 us, more than a small call's kernels.
 //
 // decode() takes exactly the calls whose arguments are valid and plain (contiguous tables,
@@ -261,10 +261,240 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// ---- paging's calls: block tables, and rows written into and read from a 4-bit cache. Each takes
+// plain calls (no output argument, contiguous vectors, the current device) and returns None for
+// the others, as decode() does; a nonzero C ABI return comes back as an int.
+
+decltype(&dk_grow_block_tables) g_grow = nullptr;
+decltype(&dk_kv4_write) g_kv4_write = nullptr;
+decltype(&dk_kv4_read) g_kv4_read = nullptr;
+
+// bind_paging(grow_block_tables, kv4_write, kv4_read: addresses), after bind()
+PyObject* bind_paging(PyObject*, PyObject* args) {
+  unsigned long long grow, write, read;
+  if (!PyArg_ParseTuple(args, "KKK", &grow, &write, &read)) return nullptr;
+  g_grow = reinterpret_cast<decltype(g_grow)>(grow);
+  g_kv4_write = reinterpret_cast<decltype(g_kv4_write)>(write);
+  g_kv4_read = reinterpret_cast<decltype(g_kv4_read)>(read);
+  Py_RETURN_NONE;
+}
+
+// A contiguous 1-D int32 or int64 tensor on dev, of n entries (any number for n < 0).
+const at::Tensor* index_arg(PyObject* o, at::Device dev, int64_t n) {
+  const at::Tensor* t = tensor_arg(o);
+  return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->dim() == 1 &&
+                 t->is_contiguous() && t->device() == dev && (n < 0 || t->size(0) == n)
+             ? t
+             : nullptr;
+}
+
+// head_dim of a 4-bit cache on a GPU, 0 for another tensor
+int64_t cache_dim(const at::Tensor* t) {
+  if (!t || t->scalar_type() != at::kByte || t->dim() != 3 || !t->device().is_cuda() ||
+      t->stride(2) != 1 || t->size(1) <= 0 || t->size(1) > INT32_MAX)
+    return 0;
+  const int64_t d = t->size(2) / 17;
+  return t->size(2) % 17 == 0 && (d == 64 || d == 128 || d == 256) ? d : 0;
+}
+
+// The raw stream of dev where it is the current device: 1; another device: 0; -1: error set.
+int stream_of(at::Device dev, void** raw) {
+  const long long cur = call_int(g_get_device, nullptr);
+  if (cur == -1 && PyErr_Occurred()) return -1;
+  if (cur != dev.index()) return 0;
+  PyObject* idx = PyLong_FromLong(dev.index());
+  PyObject* s = idx ? PyObject_CallOneArg(g_raw_stream, idx) : nullptr;
+  Py_XDECREF(idx);
+  if (!s) return -1;
+  *raw = PyLong_AsVoidPtr(s);
+  Py_DECREF(s);
+  return PyErr_Occurred() ? -1 : 1;
+}
+
+// A contiguous tensor over a part of `all`'s memory. Made directly: a view through the dispatcher
+// costs the host 0.6 us, and a step's tables are six.
+PyObject* part_of(const at::Tensor& all, int64_t offset, at::IntArrayRef sizes) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
+                                                          all.key_set(), all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return THPVariable_Wrap(std::move(t));
+}
+
+// (block_table, rows, cached_lens, new_lens, new_pages, num_tokens, capacity): the six tensors
+PyObject* grow_impl(PyObject* const* args) {
+  const at::Tensor* table = tensor_arg(args[0]);
+  if (!table || table->scalar_type() != at::kInt || table->dim() != 2 ||
+      !table->device().is_cuda() || (table->stride(1) != 1 && table->size(1) > 1) ||
+      (table->stride(0) < table->size(1) && table->size(0) > 1))
+    Py_RETURN_NONE;
+  const at::Device dev = table->device();
+  const at::Tensor* rows = index_arg(args[1], dev, -1);
+  const int64_t batch = rows ? rows->size(0) : 0;
+  if (batch <= 0 || batch >= INT32_MAX || table->size(1) > INT32_MAX) Py_RETURN_NONE;
+  const at::Tensor* cached = index_arg(args[2], dev, batch);
+  const at::Tensor* fresh = index_arg(args[3], dev, batch);
+  const at::Tensor* pages = index_arg(args[4], dev, -1);
+  int32_t tokens = 0, capacity = 0;
+  if (!cached || !fresh || !pages || pages->scalar_type() != at::kInt ||
+      !int_arg(args[5], &tokens) || !int_arg(args[6], &capacity))
+    Py_RETURN_NONE;
+  void* raw = nullptr;
+  const int on = stream_of(dev, &raw);
+  if (on < 0) return nullptr;
+  if (!on) Py_RETURN_NONE;
+  const int64_t sizes[6] = {batch + 1, capacity, batch, batch + 1, tokens, tokens};
+  int64_t total = 0;
+  for (int64_t n : sizes) total += n;
+  const at::Tensor all = at::empty({total}, table->options());
+  int32_t* base = static_cast<int32_t*>(all.data_ptr());
+  int32_t* part[6];
+  for (int i = 0; i < 6; ++i) {
+    part[i] = base;
+    base += sizes[i];
+  }
+  int rc;
+  int32_t* const td = static_cast<int32_t*>(table->data_ptr());
+  const void *rd = rows->data_ptr(), *cd = cached->data_ptr(), *nd = fresh->data_ptr();
+  const int32_t* const pd = static_cast<const int32_t*>(pages->data_ptr());
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_grow(td, table->stride(0), table->size(0), (int32_t)table->size(1), rd,
+              rows->scalar_type() == at::kLong, cd, cached->scalar_type() == at::kLong, nd,
+              fresh->scalar_type() == at::kLong, pd, pages->size(0), (int32_t)batch, part[0],
+              part[1], capacity, part[2], part[3], part[4], part[5], tokens, raw);
+  Py_END_ALLOW_THREADS
+  if (rc != DK_OK) return PyLong_FromLong(rc);
+  PyObject* out = PyTuple_New(6);
+  int64_t at = 0;
+  for (int i = 0; out && i < 6; ++i) {
+    PyObject* t = part_of(all, at, {sizes[i]});
+    at += sizes[i];
+    if (!t) Py_CLEAR(out);
+    else PyTuple_SET_ITEM(out, i, t);
+  }
+  return out;
+}
+
+// (k_new, v_new, cache, slots, q, inv_freq, positions, rope_style): 0, or the C ABI's return
+PyObject* write_impl(PyObject* const* args) {
+  const at::Tensor *k = tensor_arg(args[0]), *v = tensor_arg(args[1]), *c = tensor_arg(args[2]);
+  const int64_t d = cache_dim(c);
+  if (!k || !v || !d) Py_RETURN_NONE;
+  const at::Device dev = c->device();
+  const bool f16 = k->scalar_type() == at::kHalf;
+  if (!(f16 || k->scalar_type() == at::kBFloat16) || k->dim() != 3 || k->device() != dev ||
+      v->device() != dev || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() ||
+      v->strides() != k->strides() || k->stride(2) != 1 || k->size(0) <= 0 ||
+      k->size(1) != c->size(1) || k->size(2) != d)
+    Py_RETURN_NONE;
+  const int64_t n = k->size(0);
+  const at::Tensor* slots = index_arg(args[3], dev, n);
+  if (!slots) Py_RETURN_NONE;
+  const at::Tensor *q = nullptr, *freq = nullptr, *pos = nullptr;
+  if (args[4] != Py_None) {
+    q = tensor_arg(args[4]);
+    if (!q || q->dim() != 3 || q->size(0) != n || q->size(2) != d || q->stride(2) != 1 ||
+        q->scalar_type() != k->scalar_type() || q->device() != dev || q->size(1) > INT32_MAX)
+      Py_RETURN_NONE;
+  }
+  if (args[5] != Py_None) {
+    freq = tensor_arg(args[5]);
+    if (!freq || freq->scalar_type() != at::kFloat || freq->numel() != d / 2 ||
+        !freq->is_contiguous() || freq->device() != dev)
+      Py_RETURN_NONE;
+  }
+  if (args[6] != Py_None && !(pos = index_arg(args[6], dev, n))) Py_RETURN_NONE;
+  int32_t style = 0;
+  if (!int_arg(args[7], &style) || style > 1 || (freq && !pos)) Py_RETURN_NONE;
+  void* raw = nullptr;
+  const int on = stream_of(dev, &raw);
+  if (on < 0) return nullptr;
+  if (!on) Py_RETURN_NONE;
+  dk_strides s{};
+  if (q) {
+    s.q_b = q->stride(0);
+    s.q_h = q->stride(1);
+  }
+  s.kv_p = c->stride(0);
+  s.kv_h = c->stride(1);
+  void *qd = q ? q->data_ptr() : nullptr, *cd = c->data_ptr();
+  const void *kd = k->data_ptr(), *vd = v->data_ptr(), *sd = slots->data_ptr();
+  const void* pd = pos ? pos->data_ptr() : nullptr;
+  const float* fd = freq ? static_cast<const float*>(freq->data_ptr()) : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_kv4_write(qd, kd, vd, k->stride(0), k->stride(1), cd, sd,
+                   slots->scalar_type() == at::kLong, pd, pos && pos->scalar_type() == at::kLong,
+                   fd, style, n, q ? (int32_t)q->size(1) : 1, (int32_t)c->size(1), (int32_t)d,
+                   c->size(0), f16 ? DK_F16 : DK_BF16, &s, raw);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// (cache, slots, dtype code): (k, v)
+PyObject* read_impl(PyObject* const* args) {
+  const at::Tensor* c = tensor_arg(args[0]);
+  const int64_t d = cache_dim(c);
+  int32_t dtype = 0;
+  if (!d || !int_arg(args[2], &dtype) || (dtype != DK_F16 && dtype != DK_BF16)) Py_RETURN_NONE;
+  const at::Device dev = c->device();
+  const at::Tensor* slots = index_arg(args[1], dev, -1);
+  if (!slots || slots->size(0) <= 0) Py_RETURN_NONE;
+  void* raw = nullptr;
+  const int on = stream_of(dev, &raw);
+  if (on < 0) return nullptr;
+  if (!on) Py_RETURN_NONE;
+  const int64_t n = slots->size(0), hkv = c->size(1);
+  const at::Tensor both =
+      at::empty({2, n, hkv, d}, c->options().dtype(dtype == DK_F16 ? at::kHalf : at::kBFloat16));
+  uint8_t* const kd = static_cast<uint8_t*>(both.data_ptr());
+  uint8_t* const vd = kd + n * hkv * d * 2;
+  const void *cd = c->data_ptr(), *sd = slots->data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_kv4_read(cd, c->stride(0), c->stride(1), sd, slots->scalar_type() == at::kLong, kd, vd,
+                  hkv * d, d, n, (int32_t)hkv, (int32_t)d, c->size(0), dtype, raw);
+  Py_END_ALLOW_THREADS
+  if (rc != DK_OK) return PyLong_FromLong(rc);
+  PyObject* k = part_of(both, 0, {n, hkv, d});
+  PyObject* v = k ? part_of(both, n * hkv * d, {n, hkv, d}) : nullptr;
+  PyObject* out = v ? PyTuple_Pack(2, k, v) : nullptr;
+  Py_XDECREF(k);
+  Py_XDECREF(v);
+  return out;
+}
+
+template <PyObject* (*Impl)(PyObject* const*), int N>
+PyObject* paging_call(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != N || !g_grow || !g_get_device) {
+    PyErr_SetString(PyExc_TypeError, "_dk_native: not bound, or a wrong argument count");
+    return nullptr;
+  }
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set()) Py_RETURN_NONE;
+  try {
+    return Impl(args);
+  } catch (const std::exception&) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;   // as in decode()
+  }
+}
+
+template <PyObject* (*Impl)(PyObject* const*), int N>
+PyCFunction fast_call() {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paging_call<Impl, N>));
+}
+
 PyMethodDef kMethods[] = {
     {"bind", bind, METH_VARARGS, "addresses and callables that decode() uses"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL,
      "decode_attention's arguments by position: the output, a C ABI error code, or None"},
+    {"bind_paging", bind_paging, METH_VARARGS, "addresses that paging's calls use"},
+    {"grow_block_tables", fast_call<grow_impl, 7>(), METH_FASTCALL,
+     "grow_block_tables' arguments but out: its six tensors, a C ABI error code, or None"},
+    {"write_kv4", fast_call<write_impl, 8>(), METH_FASTCALL,
+     "write_kv4's arguments: the C ABI's return, or None"},
+    {"read_kv4", fast_call<read_impl, 3>(), METH_FASTCALL,
+     "cache, slots, dtype code: (k, v), a C ABI error code, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dk_native", nullptr, -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
