@@ -29,7 +29,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "dk_kv4.h"
+#include "dk_kernels.h"
 
 namespace dk {
 
@@ -75,20 +75,8 @@ struct ExtendArgs {
   float kscale;                        // log2(e) * softmax scale * K dequantisation scale (> 0)
   float cap_in, cap_out;               // soft-cap: x = cap_out * tanh(q.k * cap_in)
   float vscale;
-  int64_t kv_p;                        // 4-bit cache: bytes between pages (k: the pool, k_h: its kv
-                                       // heads' stride; req_to_token: page ids; num_slots: pages)
   ExtendReq req[kExtendMaxReqs];
 };
-
-// What a pool holds: q's type, fp8, or page blocks of 4 bits (dk_kv4.h)
-enum ExtendPool { kPoolSame = 0, kPoolFp8 = 1, kPoolKv4 = 2 };
-// A 4-bit row is staged in q's type at half its size (exact, the factor returned by the score scale
-// and the output's): E2M1's 6 times the largest scale of an fp16 value, 4 * 2^14, is past fp16's range.
-constexpr int kKv4StageExp = 1;
-// E8M0 byte as the float whose exponent field the widening reads, kKv4StageExp lower (255 stays NaN)
-__device__ __forceinline__ u32 kv4_stage_scale(u32 byte) {
-  return (byte == 255u ? 255u : byte - min(byte, (u32)kKv4StageExp)) << 23;
-}
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -137,14 +125,13 @@ constexpr float kExtendTop = 15.5f, kExtendMid = 8.f, kExtendJump = 14.f;
 // values of up to 2^16 times that, over any number of keys, stay far from fp32's 2^128.
 constexpr float kExtendRoom = 64.f;
 
-template <class T, int D, int POOL, bool CAP>
-__global__ __launch_bounds__(kExtendThreads, (D == 64 ? (POOL == kPoolKv4 && CAP ? 2 : 3) : D == 128 ? 2 : 1)) void dk_extend(ExtendArgs a) {
-  constexpr bool KV8 = POOL == kPoolFp8, KV4 = POOL == kPoolKv4;
+template <class T, int D, bool KV8, bool CAP>
+__global__ __launch_bounds__(kExtendThreads, (D == 64 ? 3 : D == 128 ? 2 : 1)) void dk_extend(ExtendArgs a) {
   constexpr int BN = D <= 128 ? 64 : 32;          // keys per tile
   constexpr int RB = 2 * D;                       // bytes per LDS row
   constexpr int TILE = BN * RB;
   constexpr int SCH = D * (KV8 ? 1 : 2) / 16;     // 16-byte chunks per cache row
-  constexpr int RPR = KV4 ? BN : kExtendThreads / SCH;   // rows per round of the workgroup's loads
+  constexpr int RPR = kExtendThreads / SCH;       // rows per round of the workgroup's loads
   constexpr int NR = BN / RPR;
   constexpr int KSW = (RB / 16 < 16 ? RB / 16 : 16) - 1;   // K chunk c of row t at c ^ (t & KSW)
   constexpr int VSW = (RB / 32 < 8 ? RB / 32 : 8) - 1;     // V chunk c at c ^ 2 * (t & VSW)
@@ -200,123 +187,42 @@ __global__ __launch_bounds__(kExtendThreads, (D == 64 ? (POOL == kPoolKv4 && CAP
 
   const int32_t* map = a.req_to_token + (int64_t)rq.row * a.req_stride;
   const uint8_t* kbase = a.k + (int64_t)kvh * a.k_h;
-  const uint8_t* vbase = KV4 ? kbase : a.v + (int64_t)kvh * a.v_h;
-  // a thread's part of a tile: 16-byte chunk sch of rows srow + RPR * i; of a 4-bit pool's, lane sl of
-  // 128-dim part sp of the tile's page spg (16 or, at D = 64, 8 bytes of K codes and of V codes)
+  const uint8_t* vbase = a.v + (int64_t)kvh * a.v_h;
   const int srow = tid / SCH, sch = tid % SCH;
-  const int sl = tid & 63, sp = D == 256 ? (tid >> 6) & 1 : 0, spg = tid / (D == 256 ? 128 : 64);
-  const int st = sl & 15, sr = sl >> 4;
-  constexpr int BW = D == 64 ? 2 : 4;             // 4-bit pool: words of a thread's codes
   int slot[NR];                       // of the tile whose rows are loaded next, as the map holds it
   u32x4 kr[NR], vr[NR];
-  u32 ksc = 0u, vsc = 0u;             // 4-bit pool: K's scale, the 4 scales of V's tokens
   int odd;                            // some row of kr / vr is absent or outside the pool
   auto load_slots = [&](int j) {      // past the last key: its slot again
-    if constexpr (KV4) {
-      slot[0] = map[min(j * (BN / kPage) + spg, (rq.n_all - 1) / kPage)];
-    } else {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) slot[i] = map[min(j * BN + i * RPR + srow, rq.n_all - 1)];
-    }
+    for (int i = 0; i < NR; ++i) slot[i] = map[min(j * BN + i * RPR + srow, rq.n_all - 1)];
   };
   // a slot below 0 counts from the pool's end; outside the pool, slot 0 is read instead
   auto load_tile = [&]() {
     odd = 0;
-    if constexpr (KV4) {
-      uint32_t pid = (uint32_t)slot[0];
-      if (pid >= a.num_slots) {
-        pid = 0u;
-        odd = 1;
-      }
-      const uint8_t* blk = kbase + (int64_t)pid * a.kv_p;
-      const uint8_t* kp = blk + st * (D / 2) + 4 * BW * (4 * sp + sr);
-      const uint8_t* vp = blk + kv4_v_at(D) + 1024 * sp + 4 * BW * sl;
-      if constexpr (D == 64) {
-        const u32x2 kw = *reinterpret_cast<const u32x2*>(kp), vw = *reinterpret_cast<const u32x2*>(vp);
-        kr[0] = u32x4{kw[0], kw[1], 0u, 0u};
-        vr[0] = u32x4{vw[0], vw[1], 0u, 0u};
-      } else {
-        kr[0] = *reinterpret_cast<const u32x4*>(kp);
-        vr[0] = *reinterpret_cast<const u32x4*>(vp);
-      }
-      ksc = blk[kv4_ks_at(D) + 16 * (D == 64 ? sr / 2 : 4 * sp + sr) + st];
-      vsc = *reinterpret_cast<const u32*>(blk + kv4_vs_at(D) +
-                                          16 * (D == 64 ? st / 8 : 4 * sp + st / 4) + 4 * sr);
-    } else {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        uint32_t s = (uint32_t)(slot[i] < 0 ? slot[i] + (int)a.num_slots : slot[i]);
-        if (s >= a.num_slots) {
-          s = 0u;
-          odd |= 1 << i;
-        }
-        kr[i] = *reinterpret_cast<const u32x4*>(kbase + (uint64_t)s * a.k_s + 16 * sch);
-        vr[i] = *reinterpret_cast<const u32x4*>(vbase + (uint64_t)s * a.v_s + 16 * sch);
+    for (int i = 0; i < NR; ++i) {
+      uint32_t s = (uint32_t)(slot[i] < 0 ? slot[i] + (int)a.num_slots : slot[i]);
+      if (s >= a.num_slots) {
+        s = 0u;
+        odd |= 1 << i;
       }
+      kr[i] = *reinterpret_cast<const u32x4*>(kbase + (uint64_t)s * a.k_s + 16 * sch);
+      vr[i] = *reinterpret_cast<const u32x4*>(vbase + (uint64_t)s * a.v_s + 16 * sch);
     }
   };
   // rows of keys past the request's last are zero; a row outside the pool has K = NaN, V = 0,
   // so that every query that attends to it gives NaN
   auto fix_tile = [&](int j) {
-    if constexpr (KV4) {
-      // by the scales: codes of +-0 for a zero, the NaN scale for a NaN
-      const int key = j * BN + spg * kPage;
-      const bool ka = key + st >= rq.n_all;
-      if (ka) kr[0] = u32x4{0u, 0u, 0u, 0u};
-      ksc = ka ? 127u : odd ? 255u : ksc;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bool gone = odd || key + 4 * sr + t >= rq.n_all;
-        vsc = gone ? (vsc & ~(0xffu << (8 * t))) | 127u << (8 * t) : vsc;
-        if constexpr (D == 64) {
-          vr[0][t / 2] = gone ? vr[0][t / 2] & (t & 1 ? 0xffffu : 0xffff0000u) : vr[0][t / 2];
-        } else {
-          vr[0][t] = gone ? 0u : vr[0][t];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const bool absent = j * BN + i * RPR + srow >= rq.n_all, out = odd >> i & 1;
-        const u32 fill = absent ? 0u : 0xffffffffu;
-        kr[i] = absent || out ? u32x4{fill, fill, fill, fill} : kr[i];
-        vr[i] = absent || out ? u32x4{0u, 0u, 0u, 0u} : vr[i];
-      }
+    for (int i = 0; i < NR; ++i) {
+      const bool absent = j * BN + i * RPR + srow >= rq.n_all, out = odd >> i & 1;
+      const u32 fill = absent ? 0u : 0xffffffffu;
+      kr[i] = absent || out ? u32x4{fill, fill, fill, fill} : kr[i];
+      vr[i] = absent || out ? u32x4{0u, 0u, 0u, 0u} : vr[i];
     }
   };
   auto store_tile = [&](int j, uint8_t* kt, uint8_t* vt) {
     if ((j + 1) * BN > rq.n_all || __builtin_amdgcn_ballot_w64(odd != 0)) fix_tile(j);
-    if constexpr (KV4) {
-      // K: BW * 8 dims of token st, 16-byte chunks of 8 dims
-      const int r = spg * kPage + st;
-      const u32 sc = kv4_stage_scale(ksc);
-#pragma unroll
-      for (int e = 0; e < BW; ++e) {
-        const int ch = BW * (4 * sp + sr) + e;
-        const u32 w = kr[0][e];
-        *reinterpret_cast<u32x4*>(kt + r * RB + ((ch ^ (r & KSW)) << 4)) =
-            u32x4{from_fp4<T, 0>(w, sc), from_fp4<T, 1>(w, sc), from_fp4<T, 2>(w, sc),
-                  from_fp4<T, 3>(w, sc)};
-      }
-      // V: tokens 4 sr .. 4 sr + 3, 8 dims (D = 64: 4) each
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int vr_ = spg * kPage + 4 * sr + t;
-        const u32 vs = kv4_stage_scale(vsc >> (8 * t) & 255u);
-        uint8_t* row = vt + vr_ * RB;
-        if constexpr (D == 64) {
-          const u32 w = vr[0][t / 2] >> (16 * (t & 1));
-          *reinterpret_cast<u32x2*>(row + (((st >> 1) ^ (2 * (vr_ & VSW))) << 4) + 8 * (st & 1)) =
-              u32x2{from_fp4<T, 0>(w, vs), from_fp4<T, 1>(w, vs)};
-        } else {
-          const u32 w = vr[0][t];
-          *reinterpret_cast<u32x4*>(row + (((16 * sp + st) ^ (2 * (vr_ & VSW))) << 4)) =
-              u32x4{from_fp4<T, 0>(w, vs), from_fp4<T, 1>(w, vs), from_fp4<T, 2>(w, vs),
-                    from_fp4<T, 3>(w, vs)};
-        }
-      }
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int r = i * RPR + srow;
@@ -504,9 +410,9 @@ __global__ __launch_bounds__(kExtendThreads, (D == 64 ? (POOL == kPoolKv4 && CAP
 
 // Kernel symbol of one head_dim (dk_extend.hip, compiled once per head_dim)
 template <int D>
-const void* extend_symbol(bool bf16, int pool, bool cap);
-extern template const void* extend_symbol<64>(bool, int, bool);
-extern template const void* extend_symbol<128>(bool, int, bool);
-extern template const void* extend_symbol<256>(bool, int, bool);
+const void* extend_symbol(bool bf16, bool kv8, bool cap);
+extern template const void* extend_symbol<64>(bool, bool, bool);
+extern template const void* extend_symbol<128>(bool, bool, bool);
+extern template const void* extend_symbol<256>(bool, bool, bool);
 
 }  // namespace dk

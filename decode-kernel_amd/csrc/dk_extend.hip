@@ -8,22 +8,17 @@
 
 namespace dk {
 namespace {
-template <class T, int POOL>
+template <class T, bool KV8>
 const void* sym(bool cap) {
-  return cap ? reinterpret_cast<const void*>(&dk_extend<T, DK_HEAD_DIM, POOL, true>)
-             : reinterpret_cast<const void*>(&dk_extend<T, DK_HEAD_DIM, POOL, false>);
-}
-template <class T>
-const void* sym_t(int pool, bool cap) {
-  return pool == kPoolKv4   ? sym<T, kPoolKv4>(cap)
-         : pool == kPoolFp8 ? sym<T, kPoolFp8>(cap)
-                            : sym<T, kPoolSame>(cap);
+  return cap ? reinterpret_cast<const void*>(&dk_extend<T, DK_HEAD_DIM, KV8, true>)
+             : reinterpret_cast<const void*>(&dk_extend<T, DK_HEAD_DIM, KV8, false>);
 }
 }  // namespace
 
 template <int D>
-const void* extend_symbol(bool bf16, int pool, bool cap) {
-  return bf16 ? sym_t<BF16>(pool, cap) : sym_t<F16>(pool, cap);
+const void* extend_symbol(bool bf16, bool kv8, bool cap) {
+  if (bf16) return kv8 ? sym<BF16, true>(cap) : sym<BF16, false>(cap);
+  return kv8 ? sym<F16, true>(cap) : sym<F16, false>(cap);
 }
-template const void* extend_symbol<DK_HEAD_DIM>(bool, int, bool);
+template const void* extend_symbol<DK_HEAD_DIM>(bool, bool, bool);
 }  // namespace dk

@@ -1,0 +1,467 @@
+// dk_extend_kv4.h — extend (prefill) attention over a 4-bit cache (dk_kv4.h), gfx950, wave64.
+//
+// dk_extend.h's mathematics (S^T = K.Q^T, O^T += V^T.P^T, 128 query rows of one kv head per workgroup,
+// 32 per wavefront), over page blocks found through a block table:
+//   * a wavefront loads a page's 17 D bytes a tile ahead (a quarter of 16-bit rows' traffic) and
+//     widens them to q's type on the way into LDS, in pieces between the last P.V products of the
+//     tile before, whose MFMAs leave the VALU free;
+//   * a tile's A operands are read from LDS four steps ahead of the MFMA that takes them, and its
+//     two 32-key blocks are staggered: the second's weights are formed beside the first's products;
+//   * LDS rows are padded rather than swizzled: 16 rows' 16-byte chunks (K) and 4 rows' 64-byte runs
+//     (V, transpose reads) lie in different banks, and every address is a base and a constant;
+//   * a weight enters as two parts of q's type: 22 bits in fp16 (ExtendParts<F16>), in bf16 16, off by
+//     2^-18 of itself where the output's own rounding is 2^-9 (a third part adds 1e-6 of the norm and
+//     costs 12 %).
+// Bound by the card's power where a call is long: q.k and both parts of p run at 1,120 TFLOP/s, where
+// a large library product ends at 1,305 to 1,360, and a variant with a third less MFMA work is only 16 %
+// faster, one without exponentials 7 %. 32/8/128, 2048 new of 8192 tokens, us: fp16 323, bf16 320 (dk_extend
+// over 16-bit rows 376, 441); one workgroup loop of MFMA phase, softmax, staging in turn 348, 336. 8
+// requests of 79-730 new tokens over up to 500 (32/8/64 bf16) 40: bound by the VALU and by how evenly
+// 840 workgroups of 1 to 16 key tiles fill 256 CUs.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dk_extend.h"
+#include "dk_kv4.h"
+
+namespace dk {
+
+constexpr int kKv4ExtendOrder = 512;  // query tiles of a call that it starts in an order of its own
+
+struct ExtendKv4Args {
+  ExtendArgs e;                         // k: the page pool, k_h: its kv heads' stride, req_to_token:
+                                        // page ids, num_slots: pages; vscale: undoes kv4_stage_exp
+  int64_t kv_p;                         // bytes between pages
+  int32_t ordered;                      // the tiles start in the order `order`
+  uint16_t order[kKv4ExtendOrder];
+};
+
+// Rows are staged in q's type, in fp16 at half their size (exact, the factor returned by the score
+// scale and the output's): E2M1's 6 times the largest scale of an fp16 value, 4 * 2^14, is past
+// fp16's range.
+template <class T>
+constexpr int kv4_stage_exp() { return __is_same(T, F16) ? 1 : 0; }
+// A float whose exponent field is an E8M0 byte (other bits arbitrary), halved for fp16; the NaN byte stays
+template <class T>
+__device__ __forceinline__ u32 kv4_stage_scale(u32 sc) {
+  if constexpr (kv4_stage_exp<T>() == 0) return sc;
+  return __builtin_bit_cast(u32, __builtin_bit_cast(float, sc) * 0.5f);
+}
+
+// f(Index<0>{}) .. f(Index<N - 1>{})
+template <int I>
+struct Index {
+  static constexpr int value = I;
+};
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void for_each(F&& f) {
+  if constexpr (I < N) {
+    f(Index<I>{});
+    for_each<N, I + 1>(f);
+  }
+}
+
+// x less half H of a packed pair, exact where the half is x rounded: one instruction each
+template <int H>
+__device__ __forceinline__ float less(F16, float x, u32 pair) {
+  float r;
+  if constexpr (H == 0)
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(x));
+  else
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(x));
+  return r;
+}
+template <int H>
+__device__ __forceinline__ float less(BF16, float x, u32 pair) {
+  u32 minus;   // -1 and 0, in a register: an inline -1.0 is an fp32 one
+  if constexpr (H == 0) asm("s_mov_b32 %0, 0xbf80" : "=s"(minus));
+  else asm("s_mov_b32 %0, 0xbf800000" : "=s"(minus));
+  return BF16::dot2(pair, minus, x);
+}
+
+template <class T, int D, bool CAP>
+__global__ __launch_bounds__(kExtendThreads, (D <= 128 ? 2 : 1)) void dk_extend_kv4(ExtendKv4Args ka) {
+  const ExtendArgs& a = ka.e;
+  constexpr int NB = D <= 128 ? 2 : 1;            // 32-key blocks per tile
+  constexpr int BN = 32 * NB;
+  // Bytes per LDS row, padded so that 16 rows' chunks of 16 bytes (K) and 4 rows' runs of 64 (V) fall
+  // into different banks: every offset is then a constant of the instruction
+  constexpr int KB = 2 * D + 16, VB = 2 * D + 64;
+  constexpr int KT = BN * KB, BUF = KT + BN * VB;  // K's tile, both
+  constexpr int DB = D / 32;                      // 32-dim blocks
+  constexpr int QK = D / 16;                      // q.k MFMAs per 32-key block
+  constexpr int kAhead = 4;
+  constexpr int WP = D == 256 ? 2 : 1;            // wavefronts that stage a page, 128 dims (64) each
+  constexpr int BW = D == 64 ? 2 : 4;             // words of a lane's K codes and V codes
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUF];
+  // NaN values (V's NaN scale) are staged as zeros, as 0 * NaN would reach the queries that do not
+  // attend to them; which 32-dim blocks of which tokens they were lies here, by the wavefront that
+  // staged them and where its entry of nan_tile names the tile (its number + 1)
+  __shared__ u32 nan_tile[2][4], nan_blocks[2][4][kPage];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int h = lane >> 5, c = lane & 31;
+  // workgroup -> (kv head, query tile): the kv head is fastest, so with 8 kv heads every XCD
+  // streams one head and its L2 holds that head's K and V for all tiles of a request
+  const int kvh = (int)blockIdx.x % a.hkv;
+  int t = (int)blockIdx.x / a.hkv;
+  if (ka.ordered) t = ka.order[t];
+  int lo = 0, hi = a.num_reqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.req[mid].tile0 <= t) lo = mid; else hi = mid - 1;
+  }
+  const ExtendReq rq = a.req[lo];
+  const int G = a.group, rows = rq.n_new * G;
+  // the last tiles of a request see the most keys: they start first
+  const int ntile = (rows + kExtendRows - 1) / kExtendRows;
+  const int row0 = (ntile - 1 - (t - rq.tile0)) * kExtendRows;
+  const int prefix = rq.n_all - rq.n_new;
+
+  const int rr = min(row0 + 32 * w + c, rows - 1);               // this lane's row of q
+  const int pos = prefix + rr / G;                               // and its position
+  // key range of the workgroup and of this wavefront (uniform)
+  const int wrow = min(row0 + 32 * w, rows - 1);
+  const int wpos0 = prefix + wrow / G, wpos1 = prefix + min(row0 + 32 * w + 31, rows - 1) / G;
+  const bool active = row0 + 32 * w < rows;
+  const int bpos0 = prefix + row0 / G, bpos1 = prefix + min(row0 + kExtendRows - 1, rows - 1) / G;
+  const int win = a.window > 0 ? a.window : INT32_MAX;
+  int kbeg = max(bpos0 - win + 1, 0) / BN;
+  int kend = bpos1 / BN + 1;
+  if (a.split > 1) {                   // this workgroup's range of key tiles (may be empty)
+    const int per = (kend - kbeg + a.split - 1) / a.split;
+    kbeg += (int)blockIdx.y * per;
+    kend = min(kbeg + per, kend);
+  }
+
+  u32x4 qf[QK];
+  {
+    const uint8_t* qp = a.q + (int64_t)(rq.q0 + rr / G) * a.q_b +
+                        (int64_t)(kvh * G + rr % G) * a.q_h + 16 * h;
+#pragma unroll
+    for (int i = 0; i < QK; ++i) qf[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+  }
+
+  // ---- loads: wavefront w takes page pg of the tile, part sp of its dims. Lane (sr, st): block sr
+  // (D = 64: half of one) of K token st, and dims st * W / 16 .. of V tokens 4 sr .. 4 sr + 3.
+  const int32_t* map = a.req_to_token + (int64_t)rq.row * a.req_stride;
+  const uint8_t* kbase = a.k + (int64_t)kvh * a.k_h;
+  const int pg = w / WP, sp = w % WP, st = lane & 15, sr = lane >> 4;
+  const int last_block = (rq.n_all - 1) / kPage;
+  int page = 0;                       // id that the table holds for the tile loaded next
+  bool bad = false;                   // the loaded page's id lies outside the pool
+  u32 kr[BW], vr[BW];
+  u32 ksc, vsc;                       // K's scale, V's 4 scales
+  const u32 k_off = st * (D / 2) + 64 * sp + 4 * BW * sr;
+  const u32 v_off = kv4_v_at(D) + 1024 * sp + 4 * BW * lane;
+  const u32 ks_off = kv4_ks_at(D) + 16 * (D == 64 ? sr / 2 : 4 * sp + sr) + st;
+  const u32 vs_off = kv4_vs_at(D) + 16 * (D == 64 ? st / 8 : 4 * sp + st / 4) + 4 * sr;
+  auto load_id = [&](int j) { page = map[min(j * (BN / kPage) + pg, last_block)]; };
+  auto load_tile = [&]() {            // outside the pool page 0 is read instead
+    bad = (uint32_t)uniform(page) >= a.num_slots;
+    const uint8_t* blk = kbase + (int64_t)(bad ? 0 : uniform(page)) * ka.kv_p;
+    typedef u32 Run __attribute__((ext_vector_type(BW)));
+    const Run kw = *reinterpret_cast<const Run*>(blk + k_off);
+    const Run vw = *reinterpret_cast<const Run*>(blk + v_off);
+#pragma unroll
+    for (int x = 0; x < BW; ++x) {
+      kr[x] = kw[x];
+      vr[x] = vw[x];
+    }
+    ksc = blk[ks_off];
+    vsc = *reinterpret_cast<const u32*>(blk + vs_off);
+  };
+  // keys past the request's last are zeros; a page outside the pool has K = NaN and V = 0, so that
+  // every query that attends to it gives NaN. By the scales: codes of +-0 for a zero, the NaN scale.
+  auto any_nan = [&]() {              // some scale of V is the NaN byte (a zero byte of its inverse)
+    return __builtin_amdgcn_ballot_w64(((~vsc - 0x01010101u) & vsc & 0x80808080u) != 0u) != 0u;
+  };
+  auto fix_tile = [&](int j, int buf) {
+    const int key = j * BN + pg * kPage;
+    const bool gone = key + st >= rq.n_all;
+    u32* const blocks = nan_blocks[buf != 0][w];
+    blocks[st] = 0u;
+    bool found = false;
+#pragma unroll
+    for (int x = 0; x < BW; ++x) kr[x] = gone ? 0u : kr[x];
+    ksc = gone ? 127u : bad ? 255u : ksc;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      bool out = bad || key + 4 * sr + x >= rq.n_all;
+      if (!out && (vsc >> (8 * x) & 255u) == 255u) {
+        atomicOr(&blocks[4 * sr + x], 1u << (D == 64 ? st / 8 : 4 * sp + st / 4));
+        out = found = true;
+      }
+      vsc = out ? (vsc & ~(0xffu << (8 * x))) | 127u << (8 * x) : vsc;
+      if constexpr (D == 64)
+        vr[x / 2] = out ? vr[x / 2] & (x & 1 ? 0xffffu : 0xffff0000u) : vr[x / 2];
+      else
+        vr[x] = out ? 0u : vr[x];
+    }
+    if (__builtin_amdgcn_ballot_w64(found)) nan_tile[buf != 0][w] = (u32)j + 1u;
+  };
+  // Staging, in pieces of a chunk or row: K's BW chunks of 8 dims, then V's 4 tokens
+  constexpr int PIECES = BW + 4;
+  uint8_t* const kput = smem + (pg * kPage + st) * KB + 256 * sp + 16 * BW * sr;
+  uint8_t* const vput = smem + KT + (pg * kPage + 4 * sr) * VB + 256 * sp + (D == 64 ? 8 : 16) * st;
+  auto store_piece = [&](auto piece, int buf) {
+    constexpr int p = decltype(piece)::value;
+    if constexpr (p < BW) {
+      const u32 sc = kv4_stage_scale<T>(ksc << 23);
+      *reinterpret_cast<u32x4*>(kput + buf + 16 * p) =
+          u32x4{from_fp4<T, 0>(kr[p], sc), from_fp4<T, 1>(kr[p], sc), from_fp4<T, 2>(kr[p], sc),
+                from_fp4<T, 3>(kr[p], sc)};
+    } else {
+      constexpr int x = p - BW;
+      const u32 sc = kv4_stage_scale<T>(e8m0_exp<x>(vsc));
+      if constexpr (D == 64) {
+        const u32 v = vr[x / 2] >> (16 * (x & 1));
+        *reinterpret_cast<u32x2*>(vput + buf + x * VB) =
+            u32x2{from_fp4<T, 0>(v, sc), from_fp4<T, 1>(v, sc)};
+      } else {
+        *reinterpret_cast<u32x4*>(vput + buf + x * VB) =
+            u32x4{from_fp4<T, 0>(vr[x], sc), from_fp4<T, 1>(vr[x], sc), from_fp4<T, 2>(vr[x], sc),
+                  from_fp4<T, 3>(vr[x], sc)};
+      }
+    }
+  };
+  auto store_tile = [&](int buf) {
+    for_each<PIECES>([&](auto p) { store_piece(p, buf); });
+  };
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+  float mref = kMinit, lsum = 0.f;
+  u32 nans = 0u;                      // 32-dim blocks in which this row attends to a NaN
+
+  // this lane's places in the tiles it reads (dk_extend.h)
+  const uint8_t* const kget = smem + c * KB + 16 * h;
+  const uint8_t* const vget = smem + KT + (4 * h + ((lane & 15) >> 2)) * VB +
+                              32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+
+  // A operands: 16 dims (step i) of block n's keys; 16 keys' 32 dims (step y of 2 * DB) of its V
+  auto read_k = [&](int n, int i, int buf) {
+    return *reinterpret_cast<const u32x4*>(kget + buf + 32 * n * KB + 32 * i);
+  };
+  auto read_v = [&](int n, int y, int buf) {
+    const uint8_t* vp = vget + buf + (32 * n + 16 * (y / DB)) * VB + 64 * (y % DB);
+    const u32x2 v0 = lds_read_tr(vp), v1 = lds_read_tr(vp + 8 * VB);
+    return u32x4{v0[0], v0[1], v1[0], v1[1]};
+  };
+  // pair x (0..7) of a block's weights in this lane, split into two parts
+  auto weigh = [&](int x, const f32x16& s, u32x4 (&pp)[2][2]) {
+    float r0 = __builtin_amdgcn_exp2f(CAP ? s[2 * x] - mref : __builtin_fmaf(s[2 * x], a.kscale, -mref));
+    float r1 = __builtin_amdgcn_exp2f(CAP ? s[2 * x + 1] - mref
+                                          : __builtin_fmaf(s[2 * x + 1], a.kscale, -mref));
+    lsum += r0 + r1;
+    float t0, t1;
+    const u32 top = T::pack2(r0, r1, &t0, &t1);
+    pp[x / 4][0][x % 4] = top;
+    pp[x / 4][1][x % 4] = T::pack2(less<0>(T{}, r0, top), less<1>(T{}, r1, top), &t0, &t1);
+    // computed here, beside the MFMAs around, and not where it is used first
+    asm volatile("" : "+v"(pp[x / 4][0][x % 4]), "+v"(pp[x / 4][1][x % 4]), "+v"(lsum));
+  };
+  auto pv = [&](int y, u32x4 vf, const u32x4 (&pp)[2][2]) {
+    o[y % DB] = mfma32(T{}, vf, pp[y / DB][0], o[y % DB]);
+    o[y % DB] = mfma32(T{}, vf, pp[y / DB][1], o[y % DB]);
+  };
+  // cap and mask of a block's scores; what its keys mean for `nans`
+  auto mask = [&](int k0, f32x16& s, uint64_t nan_pages, int buf) {
+    if constexpr (CAP) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = a.cap_out * tanhf(s[i] * a.cap_in);
+    }
+    if (k0 + 31 > wpos0) {
+      const int rel = pos - k0 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 > rel ? kNegInf : s[i];
+    }
+    if (k0 <= wpos1 - win) {
+      const int rel = pos - win - k0 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 <= rel ? kNegInf : s[i];
+    }
+    if (nan_pages) {
+      u32 seen = 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) seen |= s[i] != kNegInf ? 1u << i : 0u;
+#pragma unroll 1
+      for (int i = 0; i < 16; ++i) {
+        const int key = (k0 & (BN - 1)) + 8 * (i / 4) + 4 * h + i % 4;
+#pragma unroll
+        for (int x = 0; x < WP; ++x) {
+          const int from = key / kPage * WP + x;
+          if (nan_pages >> from & 1)
+            nans |= seen >> i & 1u ? nan_blocks[buf != 0][from][key % kPage] : 0u;
+        }
+      }
+    }
+  };
+  auto top_of = [&](const f32x16& s) {
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    return mx;
+  };
+  // mx, of this lane's scores: the row's; true: the reference has to move
+  auto moves = [&](float* mx) -> bool {
+    *mx = max_xor32(*mx);
+    if constexpr (!CAP) *mx *= a.kscale;
+    const bool move = ExtendParts<T>::n == 2 ? fabsf(*mx - (mref + kExtendTop / 2)) > kExtendTop / 2
+                                             : *mx > mref + kSlack;
+    return __builtin_amdgcn_ballot_w64(move);
+  };
+  auto move_ref = [&](float mx) {
+    float mn = fmaxf(mref, mx);
+    if constexpr (ExtendParts<T>::n == 2) {   // the reference follows the blocks (ExtendParts<F16>)
+      const float to = mx - (mx > mref + kExtendTop + kExtendMid ? kExtendJump : kExtendMid);
+      const float room = __builtin_amdgcn_logf(sum_xor32(lsum)) - kExtendRoom;   // log2
+      mn = mx > kNegInf ? fmaxf(to, mref + room) : mref;   // no key of the block seen: stays
+    }
+    const float al = __builtin_amdgcn_exp2f(mref - mn);
+    lsum *= al;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] *= al;
+    mref = mn;
+  };
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0x4); };   // scalar code may cross
+
+  load_id(kbeg);
+  load_tile();
+  load_id(kbeg + 1);
+  if (lane < 2) nan_tile[lane][w] = 0u;
+  if ((kbeg + 1) * BN > rq.n_all || bad || any_nan()) fix_tile(kbeg, 0);
+  store_tile(0);
+  __syncthreads();
+  for (int j = kbeg; j < kend; ++j) {
+    const int buf = (j - kbeg) & 1 ? BUF : 0;
+    load_tile();                      // after the last tile a page of the request again, for nobody
+    load_id(j + 2);
+    auto fix = [&] {
+      if ((j + 2) * BN > rq.n_all || bad || any_nan()) fix_tile(j + 1, BUF - buf);
+    };
+    // a wavefront whose rows see none of the tile's keys skips it
+    if (active && j * BN <= wpos1 && j * BN + BN - 1 > wpos0 - win) {
+      const uint64_t nan_pages =
+          __builtin_amdgcn_ballot_w64(nan_tile[buf != 0][lane & 3] == (u32)j + 1u) & 15u;
+      f32x16 s0, s1;
+      u32x4 p0[2][2], p1[2][2];
+      float mx;
+      // the tile's A operands, read kAhead steps before their use: all keys, then all values
+      u32x4 ahead[kAhead];
+      auto fetch = [&](int g) {
+        if (g < 2 * NB * QK)
+          ahead[g % kAhead] = g < NB * QK ? read_k(g / QK, g % QK, buf)
+                                          : read_v(g / QK - NB, g % QK, buf);
+      };
+#pragma unroll
+      for (int g = 0; g < kAhead; ++g) fetch(g);
+#pragma unroll
+      for (int i = 0; i < NB * QK; ++i) {
+        f32x16& x = i < QK ? s0 : s1;
+        x = mfma32(T{}, ahead[i % kAhead], qf[i % QK], i % QK ? x : f32x16{});
+        fetch(i + kAhead);
+        pin();
+      }
+      mask(j * BN, s0, nan_pages, buf);
+      mx = top_of(s0);
+      if constexpr (NB == 2) {
+        mask(j * BN + 32, s1, nan_pages, buf);
+        mx = fmaxf(mx, top_of(s1));
+      }
+      if (moves(&mx)) move_ref(mx);
+      for_each<8>([&](auto x) { weigh(x.value, s0, p0); });
+      pin();
+      if constexpr (NB == 2) {
+        // the first block's V products beside the second's weights
+        for_each<8>([&](auto x) {
+#pragma unroll
+          for (int y = x.value * QK / 8; y < (x.value + 1) * QK / 8; ++y) {
+            pv(y, ahead[(2 * QK + y) % kAhead], p0);
+            fetch(2 * QK + y + kAhead);
+          }
+          weigh(x.value, s1, p1);
+          pin();
+        });
+      }
+      // the last block's V products beside the staging of the next tile
+      fix();
+      for_each<PIECES>([&](auto p) {
+        constexpr int at = (2 * NB - 1) * QK;
+#pragma unroll
+        for (int y = p.value * QK / PIECES; y < (p.value + 1) * QK / PIECES; ++y) {
+          pv(y, ahead[(at + y) % kAhead], NB == 2 ? p1 : p0);
+          fetch(at + y + kAhead);
+        }
+        store_piece(p, BUF - buf);
+        pin();
+      });
+    } else {
+      fix();
+      store_tile(BUF - buf);
+    }
+    __syncthreads();
+  }
+
+  if (__builtin_amdgcn_ballot_w64(nans != 0u)) {
+    nans |= (u32)__shfl_xor((int)nans, 32);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = nans >> b & 1u ? __builtin_nanf("") : o[b][i];
+  }
+  lsum = sum_xor32(lsum);
+  // this lane's row again: held over the loop it would cost registers that spill
+  int base = row0;
+  asm volatile("" : "+s"(base));
+  const int row = base + 32 * w + c, tok = min(row, rows - 1) / G, head = min(row, rows - 1) - tok * G;
+  if (a.split > 1) {
+    // relative to this range's reference; dk_merge_split adds the sinks and normalises
+    if (row < rows) {
+      const int64_t r = ((int64_t)(rq.q0 + tok) * (a.hkv * G) + kvh * G + head) * a.split +
+                        blockIdx.y;
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<f32x4*>(a.part_o + r * D + 32 * b + 8 * x + 4 * h) =
+              f32x4{o[b][4 * x] * a.vscale, o[b][4 * x + 1] * a.vscale, o[b][4 * x + 2] * a.vscale,
+                    o[b][4 * x + 3] * a.vscale};
+      if (h == 0) {
+        a.part_m[r] = mref * kLn2;
+        a.part_l[r] = lsum;
+      }
+    }
+    return;
+  }
+  if (a.sinks) lsum += __builtin_amdgcn_exp2f(a.sinks[kvh * G + head] * kLog2e - mref);
+  const float inv = lsum == 0.f ? 0.f : a.vscale / lsum;
+  if (row < rows) {
+    uint8_t* op = a.out + (int64_t)(rq.q0 + tok) * a.o_b + (int64_t)(kvh * G + head) * a.o_h;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float e0, e1;
+        const u32x2 v = {T::pack2(o[b][4 * x] * inv, o[b][4 * x + 1] * inv, &e0, &e1),
+                         T::pack2(o[b][4 * x + 2] * inv, o[b][4 * x + 3] * inv, &e0, &e1)};
+        *reinterpret_cast<u32x2*>(op + 2 * (32 * b + 8 * x + 4 * h)) = v;
+      }
+  }
+}
+
+// Kernel symbol of one head_dim (dk_extend_kv4.hip, compiled once per head_dim)
+template <int D>
+const void* extend_kv4_symbol(bool bf16, bool cap);
+extern template const void* extend_kv4_symbol<64>(bool, bool);
+extern template const void* extend_kv4_symbol<128>(bool, bool);
+extern template const void* extend_kv4_symbol<256>(bool, bool);
+
+}  // namespace dk
