@@ -69,37 +69,58 @@ int check_requests(int32_t batch, const int32_t* rows, const int32_t* new_lens,
   return DK_OK;
 }
 
-// ka.order: the query tiles of all requests by their keys, most first, every second `period` of them
-// (the tiles that one workgroup per CU takes) reversed, so that a CU's workgroups have long and
-// short ones. In the order of the requests 44.0 us, so 40.4 (8 requests, 840 workgroups, 32/8/64).
-void order_tiles(ExtendKv4Args& ka, int period) {
+// Deals a call's query tiles (n of them) to `slots` workgroups per kv head, of which `period` start
+// on a CU each before the next: the longest tiles first, one per workgroup, then the next to the
+// workgroups in reverse, and so on; then the workgroups by their load, every second `period` of
+// them reversed, so that a CU's workgroups add up to much the same.
+void deal_tiles(ExtendKv4Args& ka, int n, int slots, int period) {
   const ExtendArgs& a = ka.e;
   constexpr int kLevels = 256;
-  uint16_t work[kKv4ExtendOrder];
-  int count[kLevels + 1] = {};
+  int32_t load[kKv4ExtendOrder] = {};
+  uint16_t work[kKv4ExtendOrder], tile[kKv4ExtendOrder], rank[kKv4ExtendOrder];
+  // ranks of `count` items by falling size
+  auto sort = [&](const auto* size, int count, int64_t most) {
+    int at[kLevels + 1] = {};
+    auto level = [&](int i) { return kLevels - 1 - (int)((int64_t)size[i] * (kLevels - 1) / most); };
+    for (int i = 0; i < count; ++i) ++at[level(i) + 1];
+    for (int i = 0; i < kLevels; ++i) at[i + 1] += at[i];
+    for (int i = 0; i < count; ++i) rank[i] = (uint16_t)at[level(i)]++;
+  };
   int64_t most = 1;
-  for (int r = 0; r < a.num_reqs; ++r) most = std::max<int64_t>(most, a.req[r].n_all);
-  int n = 0;
-  for (int r = 0; r < a.num_reqs; ++r) {
+  for (int r = 0, i = 0; r < a.num_reqs; ++r) {
     const ExtendReq& q = a.req[r];
     const int64_t rows = (int64_t)q.n_new * a.group;
     const int tiles = (int)((rows + kExtendRows - 1) / kExtendRows);
-    for (int k = 0; k < tiles; ++k, ++n) {         // the kernel starts a request's last tile first
+    for (int k = 0; k < tiles; ++k, ++i) {         // a request's n-th tile counts from its end
       const int64_t row0 = (int64_t)(tiles - 1 - k) * kExtendRows;
       const int64_t last = std::min(row0 + kExtendRows, rows) - 1;
       int64_t keys = q.n_all - q.n_new + last / a.group + 1;
       if (a.window > 0) keys = std::min<int64_t>(keys, a.window + kExtendRows / a.group + 1);
-      const int level = (int)(kLevels - 1 - keys * (kLevels - 1) / most);
-      work[n] = (uint16_t)level;
-      ++count[level + 1];
+      work[i] = (uint16_t)std::min<int64_t>(keys / 32 + 2, 32767);   // and a tile's fixed cost
+      tile[i] = (uint16_t)(r * kKv4ExtendOrder + k);
+      most = std::max<int64_t>(most, work[i]);
     }
   }
-  for (int i = 0; i < kLevels; ++i) count[i + 1] += count[i];
+  sort(work, n, most);
+  uint16_t owner[kKv4ExtendOrder], next[kKv4ExtendOrder] = {};
+  most = 1;
   for (int i = 0; i < n; ++i) {
-    const int at = count[work[i]]++;
-    const int round = at / period, first = round * period;
-    const int end = std::min(first + period, n);
-    ka.order[round & 1 ? end - 1 - (at - first) : at] = (uint16_t)i;
+    const int turn = rank[i] / slots, x = rank[i] % slots;
+    owner[i] = (uint16_t)(turn & 1 ? slots - 1 - x : x);
+    load[owner[i]] += work[i];
+    most = std::max<int64_t>(most, load[owner[i]]);
+  }
+  sort(load, slots, most);
+  for (int i = 0; i < slots; ++i) {
+    const int first = rank[i] / period * period, end = std::min(first + period, slots);
+    if (rank[i] / period & 1) rank[i] = (uint16_t)(end - 1 - (rank[i] - first));
+  }
+  for (int i = 0; i <= slots; ++i) ka.start[i] = 0;
+  for (int i = 0; i < n; ++i) ++ka.start[rank[owner[i]] + 1];
+  for (int i = 0; i < slots; ++i) ka.start[i + 1] += ka.start[i];
+  for (int i = 0; i < n; ++i) {
+    const int x = rank[owner[i]];
+    ka.list[ka.start[x] + next[x]++] = tile[i];
   }
 }
 
@@ -143,13 +164,18 @@ int launch_extend(ExtendArgs& a, ExtendKv4Args* kv4, const void* fn, const int32
     if (n == 0) break;
     a.num_reqs = n;
     a.tiles = (int32_t)tiles;
+    int64_t slots = tiles;
     if (kv4) {
-      kv4->ordered = a.split == 1 && n > 1 && tiles <= kKv4ExtendOrder;
-      if (kv4->ordered) order_tiles(*kv4, std::max(256 / a.hkv, 1));
+      const int period = std::max(256 / a.hkv, 1);
+      kv4->dealt = a.split == 1 && tiles <= kKv4ExtendOrder;
+      if (kv4->dealt) {
+        slots = std::min<int64_t>(tiles, kv4_extend_resident(head_dim, a.cap_out != 0.f) * period);
+        deal_tiles(*kv4, (int)tiles, (int)slots, period);
+      }
     }
     void* args[] = {kv4 ? (void*)kv4 : (void*)&a};
     const hipError_t e =
-        hipLaunchKernel(fn, dim3((uint32_t)(tiles * a.hkv), a.split), dim3(kExtendThreads), args, 0,
+        hipLaunchKernel(fn, dim3((uint32_t)(slots * a.hkv), a.split), dim3(kExtendThreads), args, 0,
                         static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return set_error((int)e, "extend launch: %s", hipGetErrorString(e));
   }

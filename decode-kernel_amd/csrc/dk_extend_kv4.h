@@ -14,10 +14,12 @@
 //     costs 12 %).
 // Bound by the card's power where a call is long: q.k and both parts of p run at 1,120 TFLOP/s, where
 // a large library product ends at 1,305 to 1,360, and a variant with a third less MFMA work is only 16 %
-// faster, one without exponentials 7 %. 32/8/128, 2048 new of 8192 tokens, us: fp16 323, bf16 320 (dk_extend
+// faster, one without exponentials 7 %. 32/8/128, 2048 new of 8192 tokens, us: fp16 323, bf16 318 (dk_extend
 // over 16-bit rows 376, 441); one workgroup loop of MFMA phase, softmax, staging in turn 348, 336. 8
-// requests of 79-730 new tokens over up to 500 (32/8/64 bf16) 40: bound by the VALU and by how evenly
-// 840 workgroups of 1 to 16 key tiles fill 256 CUs.
+// requests of 79-730 new tokens over up to 500 (32/8/64 bf16) 38.6: bound by the VALU, 1.0 us per
+// workgroup and 64-key tile on a CU that holds three, and by the longest workgroup, 16 tiles of
+// 1.75 us. Tiles dealt to the workgroups that the chip holds (ExtendKv4Args) against one workgroup
+// per tile: 38.6 and 42.6, one request of 2048 tokens (32/8/128 fp16) 65.3 and 67.8.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -28,14 +30,19 @@
 
 namespace dk {
 
-constexpr int kKv4ExtendOrder = 512;  // query tiles of a call that it starts in an order of its own
+constexpr int kKv4ExtendOrder = 256;  // query tiles that a call deals out itself (ExtendKv4Args)
+
+// Workgroups that a CU holds at once
+constexpr int kv4_extend_resident(int d, bool cap) { return d == 64 ? (cap ? 2 : 3) : d == 128 ? 2 : 1; }
 
 struct ExtendKv4Args {
   ExtendArgs e;                         // k: the page pool, k_h: its kv heads' stride, req_to_token:
                                         // page ids, num_slots: pages; vscale: undoes kv4_stage_exp
   int64_t kv_p;                         // bytes between pages
-  int32_t ordered;                      // the tiles start in the order `order`
-  uint16_t order[kKv4ExtendOrder];
+  // dealt != 0: a workgroup takes the query tiles list[start[i]] .. list[start[i + 1] - 1] of its
+  // head, i = its index in the grid; a tile: request * kKv4ExtendOrder + its n-th tile
+  int32_t dealt;
+  uint16_t list[kKv4ExtendOrder], start[kKv4ExtendOrder + 1];
 };
 
 // Rows are staged in q's type, in fp16 at half their size (exact, the factor returned by the score
@@ -82,7 +89,7 @@ __device__ __forceinline__ float less(BF16, float x, u32 pair) {
 }
 
 template <class T, int D, bool CAP>
-__global__ __launch_bounds__(kExtendThreads, (D <= 128 ? 2 : 1)) void dk_extend_kv4(ExtendKv4Args ka) {
+__global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void dk_extend_kv4(ExtendKv4Args ka) {
   const ExtendArgs& a = ka.e;
   constexpr int NB = D <= 128 ? 2 : 1;            // 32-key blocks per tile
   constexpr int BN = 32 * NB;
@@ -101,23 +108,35 @@ __global__ __launch_bounds__(kExtendThreads, (D <= 128 ? 2 : 1)) void dk_extend_
   // staged them and where its entry of nan_tile names the tile (its number + 1)
   __shared__ u32 nan_tile[2][4], nan_blocks[2][4][kPage];
 
-  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
-  const int h = lane >> 5, c = lane & 31;
   // workgroup -> (kv head, query tile): the kv head is fastest, so with 8 kv heads every XCD
   // streams one head and its L2 holds that head's K and V for all tiles of a request
   const int kvh = (int)blockIdx.x % a.hkv;
-  int t = (int)blockIdx.x / a.hkv;
-  if (ka.ordered) t = ka.order[t];
-  int lo = 0, hi = a.num_reqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.req[mid].tile0 <= t) lo = mid; else hi = mid - 1;
+  const int t = (int)blockIdx.x / a.hkv;
+  int entry = ka.dealt ? ka.start[t] : 0;
+  const int entries = ka.dealt ? ka.start[t + 1] : 1;
+  do {
+  // the lane's places, formed again for each tile: held from one to the next they would spill
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, w = uniform(tid >> 6);
+  const int h = lane >> 5, c = lane & 31;
+  int lo = 0, nth;                     // the request, and which of its tiles
+  if (ka.dealt) {
+    lo = ka.list[entry] / kKv4ExtendOrder;
+    nth = ka.list[entry] % kKv4ExtendOrder;
+  } else {
+    int hi = a.num_reqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.req[mid].tile0 <= t) lo = mid; else hi = mid - 1;
+    }
+    nth = t - a.req[lo].tile0;
   }
   const ExtendReq rq = a.req[lo];
   const int G = a.group, rows = rq.n_new * G;
   // the last tiles of a request see the most keys: they start first
   const int ntile = (rows + kExtendRows - 1) / kExtendRows;
-  const int row0 = (ntile - 1 - (t - rq.tile0)) * kExtendRows;
+  const int row0 = (ntile - 1 - nth) * kExtendRows;
   const int prefix = rq.n_all - rq.n_new;
 
   const int rr = min(row0 + 32 * w + c, rows - 1);               // this lane's row of q
@@ -439,7 +458,7 @@ __global__ __launch_bounds__(kExtendThreads, (D <= 128 ? 2 : 1)) void dk_extend_
         a.part_l[r] = lsum;
       }
     }
-    return;
+    return;                            // such a call deals nothing out
   }
   if (a.sinks) lsum += __builtin_amdgcn_exp2f(a.sinks[kvh * G + head] * kLog2e - mref);
   const float inv = lsum == 0.f ? 0.f : a.vscale / lsum;
@@ -455,6 +474,7 @@ __global__ __launch_bounds__(kExtendThreads, (D <= 128 ? 2 : 1)) void dk_extend_
         *reinterpret_cast<u32x2*>(op + 2 * (32 * b + 8 * x + 4 * h)) = v;
       }
   }
+  } while (++entry < entries);
 }
 
 // Kernel symbol of one head_dim (dk_extend_kv4.hip, compiled once per head_dim)

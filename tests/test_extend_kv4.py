@@ -193,6 +193,33 @@ def test_what_lies_behind_a_request_is_not_read_and_bad_pages_give_nan(d, dtype)
     assert np.isnan(got[:23, 2:]).all() and np.isfinite(got[:23, :2]).all() and np.isfinite(got[23:-1]).all()
 
 
+# More query tiles than workgroups that the chip holds per kv head, so that workgroups take several;
+# more than a call deals out; more requests than a launch takes
+MANY = [
+    ([(0, 300), (7, 129), (64, 1), (0, 0), (33, 260), (5, 40), (0, 513)], 64, 64, 64),
+    ([(0, 300), (7, 129), (64, 1), (33, 260)], 100, 50, 128), ([(9, 257), (0, 140)], 60, 60, 256),
+    ([(0, 140), (3, 129)], 300, 300, 64), ([(i % 50, 1 + i % 3) for i in range(270)], 4, 2, 64),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reqs,hq,hkv,d", MANY)
+def test_many_tiles(reqs, hq, hkv, d):
+    q, cache, raw, table, rows, new, alls = _case(reqs, hq, hkv, d, torch.bfloat16, hq)
+    t = torch.from_numpy(table).to(DEV)
+    for window in (0, 70):
+        out = torch.full_like(q, 7.0)
+        got = extend.extend_attention_kv4(q, cache, t, rows, new, alls, out=out, window=window or None)
+        assert got is out and bool((out[sum(new):] == 7.0).all())
+        some, g = sorted({0, hkv // 2, hkv - 1}), hq // hkv    # kv heads, and their q heads
+        heads = [x * g + i for x in some for i in range(g)]
+        want, size, big = _oracle(to_np(q[:, heads].double()), raw[:, some], table, rows, new, alls, window)
+        _check(got[:-1, heads], want[:-1], size, big, torch.bfloat16)
+        for _ in range(2):
+            again = extend.extend_attention_kv4(q, cache, t, rows, new, alls, window=window or None)
+            assert torch.equal(again[:-1], got[:-1])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("d", [64, 128, 256])
