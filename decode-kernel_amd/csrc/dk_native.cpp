@@ -141,7 +141,8 @@ PyObject* decode_impl(PyObject* const* args) {
   if (args[kWindow] != Py_None && !int_arg(args[kWindow], &o.window)) Py_RETURN_NONE;
   bool given = false;
   if (!positive_arg(args[kSmScale], &given, &o.sm_scale)) Py_RETURN_NONE;
-  if (!positive_arg(args[kLogitCap], &given, &o.logit_cap)) Py_RETURN_NONE;
+  const bool no_cap = PyFloat_CheckExact(args[kLogitCap]) && PyFloat_AS_DOUBLE(args[kLogitCap]) == 0.0;
+  if (!no_cap && !positive_arg(args[kLogitCap], &given, &o.logit_cap)) Py_RETURN_NONE;
   float scale[2] = {1.f, 1.f};
   for (int i = 0; i < 2; ++i) {
     if (!positive_arg(args[kKScale + i], &given, &scale[i])) Py_RETURN_NONE;
