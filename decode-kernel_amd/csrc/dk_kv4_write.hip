@@ -8,9 +8,12 @@
 // that the next scale has). Codes are x / scale rounded to the nearest, ties to the even code. A
 // block with a NaN or an infinity gets the NaN scale, so that it reads as NaN.
 //
-// Rotation as in dk_append_kv (rotate-half pairs or interleaved ones, fp32, one rounding of q), but
-// for the angle: position * inv_freq is formed in double and reduced in turns, so that a position of
-// 100,000 keeps the fp32 accuracy of a near one (an fp32 product of 1e5 is off by up to 4e-3).
+// Rotation as in dk_append_kv (rotate-half pairs or interleaved ones, one rounding of q), but for the
+// angle: position * inv_freq is formed and reduced in double, so that a position of 100,000 keeps the
+// accuracy of a near one (an fp32 product of 1e5 is off by up to 4e-3). q is rotated in fp32, K in
+// double: an fp32 rotation puts about one K element of 8 million on the other side of a boundary
+// between two codes, a whole step of E2M1 away. Bound by memory: 8192 tokens of 32/8/128 40.8 us (176
+// MB, 4.3 TB/s, where a large copy reaches 4.9), with K in fp32 too 38.5.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -25,9 +28,11 @@ namespace dk {
 namespace {
 
 constexpr int kWriteThreads = 256;
-// From this many tokens on a workgroup takes several, fewer than fill the chip take one each.
-constexpr int64_t kWriteManyTokens = 4096;
-constexpr int kWriteGroupTokens = 4;
+// From this many tokens on a workgroup takes several (its angles serve more rows and its loads overlap:
+// 8192 tokens of 32/8/128, us, 2 / 4 / 8 tokens 44.3 / 41.4 / 40.8; 16384 of 32/8/64 54.4 / 49.0 / 46.3);
+// fewer take one each, their rows over as many workgroups as they fill.
+constexpr int64_t kWriteManyTokens = 8192;
+constexpr int kWriteGroupTokens = 8;
 
 struct Kv4WriteArgs {
   uint8_t* q;                 // may be null
@@ -47,31 +52,47 @@ struct Kv4WriteArgs {
   int32_t per_group;          // tokens per workgroup
 };
 
-// (cos, sin) of position * f: whole turns leave in double (exact product, error 2^-52 of the
-// turns), then a quarter turn's polynomial: Taylor series to x^11 / x^12 over |x| <= pi/4, off by
-// less than 1e-9 before rounding.
-__device__ __forceinline__ void cos_sin(double position, float f, float* cs, float* sn) {
-  const double turns = position * (double)f * 0.15915494309189535;
-  const double part = turns - __builtin_rint(turns);         // in [-1/2, 1/2]
-  const double quarter = __builtin_rint(part * 4.0);         // -2 .. 2
-  const float x = (float)((part - 0.25 * quarter) * 6.283185307179586);
-  const float x2 = x * x;
-  float s = -2.5052108e-8f, c = 2.0876757e-9f;               // -1/11!, 1/12!
-  s = __builtin_fmaf(s, x2, 2.7557319e-6f);
-  s = __builtin_fmaf(s, x2, -1.9841270e-4f);
-  s = __builtin_fmaf(s, x2, 8.3333333e-3f);
-  s = __builtin_fmaf(s, x2, -1.6666667e-1f);
-  s = __builtin_fmaf(s * x2, x, x);
-  c = __builtin_fmaf(c, x2, -2.7557319e-7f);
-  c = __builtin_fmaf(c, x2, 2.4801587e-5f);
-  c = __builtin_fmaf(c, x2, -1.3888889e-3f);
-  c = __builtin_fmaf(c, x2, 4.1666667e-2f);
-  c = __builtin_fmaf(c, x2, -0.5f);
-  c = __builtin_fmaf(c, x2, 1.0f);
-  const int n = (int)quarter & 3;
-  const float a = n & 1 ? s : c, b = n & 1 ? c : s;          // |cos|, |sin| of the quadrant
+// (cos, sin) of position * f in double: the product is exact, quarter turns leave it in two parts of
+// pi / 2 (the second what the first lacks of it), then the Taylor series to x^16 / x^17 over
+// |x| <= pi / 4, off by less than 1e-16.
+__device__ __forceinline__ void cos_sin(double position, float f, double* cs, double* sn) {
+  const double angle = position * (double)f;
+  const double quarter = __builtin_rint(angle * 0.6366197723675814);   // 2 / pi
+  const double x = __builtin_fma(-quarter, 6.123233995736766e-17,
+                                 __builtin_fma(-quarter, 1.5707963267948966, angle));
+  const double x2 = x * x;
+  double s = 2.8114572543455206e-15, c = 4.779477332387385e-14;        // 1/17!, 1/16!
+  s = __builtin_fma(s, x2, -7.647163731819816e-13);
+  s = __builtin_fma(s, x2, 1.6059043836821613e-10);
+  s = __builtin_fma(s, x2, -2.505210838544172e-08);
+  s = __builtin_fma(s, x2, 2.7557319223985893e-06);
+  s = __builtin_fma(s, x2, -1.984126984126984e-04);
+  s = __builtin_fma(s, x2, 8.333333333333333e-03);
+  s = __builtin_fma(s, x2, -1.6666666666666666e-01);
+  s = __builtin_fma(s * x2, x, x);
+  c = __builtin_fma(c, x2, -1.1470745597729725e-11);
+  c = __builtin_fma(c, x2, 2.08767569878681e-09);
+  c = __builtin_fma(c, x2, -2.755731922398589e-07);
+  c = __builtin_fma(c, x2, 2.48015873015873e-05);
+  c = __builtin_fma(c, x2, -1.388888888888889e-03);
+  c = __builtin_fma(c, x2, 4.1666666666666664e-02);
+  c = __builtin_fma(c, x2, -0.5);
+  c = __builtin_fma(c, x2, 1.0);
+  const int n = (int)((int64_t)quarter & 3);
+  const double a = n & 1 ? s : c, b = n & 1 ? c : s;         // |cos|, |sin| of the quadrant
   *cs = n == 1 || n == 2 ? -a : a;
   *sn = n >= 2 ? -b : b;
+}
+
+// y in fp32 such that a rounding to fewer bits gives what it gives for y: cut towards zero, the last
+// bit set where something was cut (NaN and infinities stay)
+__device__ __forceinline__ float to_odd(double y) {
+  const float f = (float)y;
+  const double back = f;
+  u32 b = __builtin_bit_cast(u32, f);
+  b -= __builtin_fabs(back) > __builtin_fabs(y) ? 1u : 0u;
+  b |= back != y ? 1u : 0u;
+  return __builtin_bit_cast(float, b);
 }
 
 template <class E>
@@ -121,20 +142,39 @@ __device__ __forceinline__ int64_t index_at(const void* p, int32_t wide, int64_t
   return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
+// turn(f, p, q, &u, &v) for the pairs (p, q) of two runs of 8 dims from i0 and i1: across them (style
+// 0), or neighbours within each; f: the pair's frequency
+template <class F>
+__device__ __forceinline__ void turn_pairs(int style, int i0, int i1, float (&y0)[8], float (&y1)[8],
+                                           F&& turn) {
+  if (style == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      turn(i0 + e, y0[e], y1[e], &y0[e], &y1[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      turn(i0 / 2 + e / 2, y0[e], y0[e + 1], &y0[e], &y0[e + 1]);
+      turn(i1 / 2 + e / 2, y1[e], y1[e + 1], &y1[e], &y1[e + 1]);
+    }
+  }
+}
+
 // Workgroup: per_group consecutive tokens (blockIdx.x), slice blockIdx.y of their units. A unit is 8
-// + 8 dims of one q or K head (its pairs), or 8 dims of a V head; 4 neighbouring lanes hold a block's
-// 32 dims. The tokens' cosines and sines are formed once, in LDS, for all heads. With inv_freq and q null
-// the K rows are written as they are.
+// + 8 dims of one head's row (a rotated one's pairs); 4 neighbouring lanes hold a block's 32 dims. The
+// tokens' cosines and sines are formed once, in LDS, for all heads. Without inv_freq q is left alone
+// and K is written as it is.
 template <class E, int D>
 __global__ __launch_bounds__(kWriteThreads) void dk_kv4_write_kernel(Kv4WriteArgs a) {
   constexpr int HU = D / 16;                                 // units of a q or K head
-  constexpr int VU = D / 8;
-  extern __shared__ float trig[];                            // per token: D/2 cosines, D/2 sines
+  extern __shared__ __attribute__((aligned(8))) float trig[];   // per token: D/2 cosines, D/2 sines;
+  double* const trig64 = reinterpret_cast<double*>(trig + a.per_group * D);   // the same in double
   const int t0 = blockIdx.x * a.per_group;
   const int nt = min(a.per_group, a.tokens - t0);
   const bool rot = a.inv_freq != nullptr;
   const int qu = a.q && rot ? a.hq * HU : 0, ku = a.hkv * HU;
-  const int units = qu + ku + a.hkv * VU;
+  const int units = qu + 2 * ku;
 
   auto where = [&](int t, int* slot, int64_t* pos) -> uint8_t* {
     *slot = 0;
@@ -156,91 +196,116 @@ __global__ __launch_bounds__(kWriteThreads) void dk_kv4_write_kernel(Kv4WriteArg
     return page < a.num_pages ? a.cache + (int64_t)page * a.kv_p : nullptr;
   };
 
+  // two runs of 8 dims of a row: rotated pairs lie across them (rotate half) or inside (interleaved)
+  struct Unit {
+    int t, x;                                                // token of the group, unit of the token
+    Run8<E> lo, hi;
+  };
+  auto row_of = [&](const Unit& u) -> uint8_t* {
+    const int h = (u.x < qu ? u.x : u.x < qu + ku ? u.x - qu : u.x - qu - ku) / HU;
+    const int64_t t = t0 + u.t;
+    if (u.x < qu) return a.q + t * a.q_b + (int64_t)h * a.q_h;
+    return const_cast<uint8_t*>(u.x < qu + ku ? a.k_new : a.v_new) + t * a.n_b + (int64_t)h * a.n_h;
+  };
+  auto fetch = [&](int at, Unit& u) {
+    u.t = at / units;
+    u.x = at - u.t * units;
+    const uint8_t* row = row_of(u) + 16 * (u.x % HU);        // qu and ku are multiples of HU
+    u.lo = *reinterpret_cast<const Run8<E>*>(row);
+    u.hi = *reinterpret_cast<const Run8<E>*>(row + D);
+  };
+  Unit u0, u1;
+  const int first = blockIdx.y * kWriteThreads + threadIdx.x;
+  if (first < nt * units) fetch(first, u0);                  // in flight while the angles are formed
   if (rot) {
     for (int i = threadIdx.x; i < nt * (D / 2); i += kWriteThreads) {
       const int t = i / (D / 2), f = i % (D / 2);
       int slot;
       int64_t pos;
       where(t0 + t, &slot, &pos);
-      float c, s;
+      double c, s;
       cos_sin((double)pos, a.inv_freq[f], &c, &s);
-      trig[t * D + f] = c;
-      trig[t * D + D / 2 + f] = s;
+      trig[t * D + f] = (float)c;
+      trig[t * D + D / 2 + f] = (float)s;
+      trig64[t * D + f] = c;
+      trig64[t * D + D / 2 + f] = s;
     }
     __syncthreads();
   }
-  for (int u = blockIdx.y * kWriteThreads + threadIdx.x; u < nt * units;
-       u += gridDim.y * kWriteThreads) {
-    const int tl = u / units, t = t0 + tl;
-    int x = u - tl * units;
+  auto put = [&](const Unit& u) {
+    const int t = t0 + u.t, x = u.x, n = x % HU;
+    const int i0 = 8 * n, i1 = 8 * n + D / 2;
+    const bool is_q = x < qu, is_k = !is_q && x < qu + ku;
     int slot;
     uint8_t* blk = where(t, &slot, nullptr);
     // a sequence without pages has no token to append: its q row stays (as in dk_append_kv)
-    const bool none = !a.slots && a.indptr[t + 1] <= a.indptr[t];
-    if (x < qu + ku) {
-      const bool is_q = x < qu;
-      if (!is_q) x -= qu;
-      const int h = x / HU, n = x % HU;                      // head, 8-pair column
-      uint8_t* row = is_q ? a.q + (int64_t)t * a.q_b + (int64_t)h * a.q_h
-                          : const_cast<uint8_t*>(a.k_new) + (int64_t)t * a.n_b + (int64_t)h * a.n_h;
-      // two runs of 8 dims: their pairs lie across them (rotate half) or inside (interleaved)
-      const int i0 = 8 * n, i1 = 8 * n + D / 2;
-      const Run8<E> lo = *reinterpret_cast<const Run8<E>*>(row + 2 * i0);
-      const Run8<E> hi = *reinterpret_cast<const Run8<E>*>(row + 2 * i1);
-      float y0[8], y1[8];
+    if (is_q ? !a.slots && a.indptr[t + 1] <= a.indptr[t] : !blk) return;
+    const int tl = u.t;
+    const Run8<E> &lo = u.lo, &hi = u.hi;
+    float y0[8], y1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y0[e] = (float)lo[e];
+      y1[e] = (float)hi[e];
+    }
+    if (rot && is_q) {
+      const float *cs = trig + tl * D, *sn = cs + D / 2;
+      turn_pairs(a.rope_style, i0, i1, y0, y1, [&](int f, float p, float q, float* u, float* v) {
+        *u = __builtin_fmaf(p, cs[f], -(q * sn[f]));
+        *v = __builtin_fmaf(p, sn[f], q * cs[f]);
+      });
+    } else if (rot && is_k) {
+      const double *cs = trig64 + tl * D, *sn = cs + D / 2;
+      turn_pairs(a.rope_style, i0, i1, y0, y1, [&](int f, double p, double q, float* u, float* v) {
+        *u = (float)(p * cs[f] - q * sn[f]);
+        *v = (float)(p * sn[f] + q * cs[f]);
+      });
+      // every boundary between codes, and between scales, is a float of at most 2 mantissa bits: only
+      // one that came out as such may lie on its other side
+      u32 low = ~0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        low = min(low, min(__builtin_bit_cast(u32, y0[e]) & 0x1fffffu,
+                           __builtin_bit_cast(u32, y1[e]) & 0x1fffffu));
+      if (__builtin_amdgcn_ballot_w64(low == 0u)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y0[e] = (float)lo[e];
+          y1[e] = (float)hi[e];
+        }
+        turn_pairs(a.rope_style, i0, i1, y0, y1, [&](int f, double p, double q, float* u, float* v) {
+          *u = to_odd(p * cs[f] - q * sn[f]);
+          *v = to_odd(p * sn[f] + q * cs[f]);
+        });
+      }
+    }
+    if (is_q) {
+      Run8<E> o0, o1;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        y0[e] = (float)lo[e];
-        y1[e] = (float)hi[e];
+        o0[e] = (E)y0[e];
+        o1[e] = (E)y1[e];
       }
-      if (rot) {
-        const float* cs = trig + tl * D;
-        const float* sn = cs + D / 2;
-        if (a.rope_style == 0) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float c = cs[i0 + e], s = sn[i0 + e], p = y0[e], q = y1[e];
-            y0[e] = __builtin_fmaf(p, c, -(q * s));
-            y1[e] = __builtin_fmaf(p, s, q * c);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float c0 = cs[i0 / 2 + e / 2], s0 = sn[i0 / 2 + e / 2];
-            const float c1 = cs[i1 / 2 + e / 2], s1 = sn[i1 / 2 + e / 2];
-            const float p0 = y0[e], q0 = y0[e + 1], p1 = y1[e], q1 = y1[e + 1];
-            y0[e] = __builtin_fmaf(p0, c0, -(q0 * s0));
-            y0[e + 1] = __builtin_fmaf(p0, s0, q0 * c0);
-            y1[e] = __builtin_fmaf(p1, c1, -(q1 * s1));
-            y1[e + 1] = __builtin_fmaf(p1, s1, q1 * c1);
-          }
-        }
-      }
-      if (is_q) {
-        if (!none) {
-          Run8<E> o0, o1;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o0[e] = (E)y0[e];
-            o1[e] = (E)y1[e];
-          }
-          *reinterpret_cast<Run8<E>*>(row + 2 * i0) = o0;
-          *reinterpret_cast<Run8<E>*>(row + 2 * i1) = o1;
-        }
-      } else if (blk) {                                      // the same for a block's 4 lanes
-        put8<D, false>(blk + (int64_t)h * a.kv_h, slot, i0, y0);
-        put8<D, false>(blk + (int64_t)h * a.kv_h, slot, i1, y1);
-      }
-    } else if (blk) {
-      x -= qu + ku;
-      const int h = x / VU, i = 8 * (x % VU);
-      const Run8<E> v = *reinterpret_cast<const Run8<E>*>(a.v_new + (int64_t)t * a.n_b +
-                                                          (int64_t)h * a.n_h + 2 * i);
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (float)v[e];
-      put8<D, true>(blk + (int64_t)h * a.kv_h, slot, i, y);
+      uint8_t* row = row_of(u);
+      *reinterpret_cast<Run8<E>*>(row + 2 * i0) = o0;
+      *reinterpret_cast<Run8<E>*>(row + 2 * i1) = o1;
+    } else if (is_k) {                                       // the same for a block's 4 lanes
+      blk += (int64_t)((x - qu) / HU) * a.kv_h;
+      put8<D, false>(blk, slot, i0, y0);
+      put8<D, false>(blk, slot, i1, y1);
+    } else {
+      blk += (int64_t)((x - qu - ku) / HU) * a.kv_h;
+      put8<D, true>(blk, slot, i0, y0);
+      put8<D, true>(blk, slot, i1, y1);
     }
+  };
+  // the next unit's rows are in flight while one is put
+  const int step = gridDim.y * kWriteThreads, all = nt * units;
+  for (int at = first; at < all; at += 2 * step) {
+    if (at + step < all) fetch(at + step, u1);
+    put(u0);
+    if (at + 2 * step < all) fetch(at + 2 * step, u0);
+    if (at + step < all) put(u1);
   }
 }
 
@@ -369,14 +434,14 @@ int write_impl(const char* what, void* q, const void* k_new, const void* v_new, 
   a.num_pages = (uint32_t)std::min<int64_t>(num_pages, (int64_t)1 << 31);
   // few tokens: one per workgroup, its units over as many workgroups as they fill; many: several
   // tokens per workgroup
-  const int64_t units = (int64_t)(q && a.inv_freq ? hq : 0) * (d / 16) + (int64_t)hkv * (d / 16 + d / 8);
+  const int64_t units = ((int64_t)(q && a.inv_freq ? hq : 0) + 2 * (int64_t)hkv) * (d / 16);
   a.per_group = tokens >= kWriteManyTokens ? kWriteGroupTokens : 1;
   const int64_t groups = (tokens + a.per_group - 1) / a.per_group;
   const int64_t slices = a.per_group > 1 ? 1 : (units + kWriteThreads - 1) / kWriteThreads;
   void* args[] = {&a};
   const hipError_t e = hipLaunchKernel(
       write_symbol(dtype, d), dim3((uint32_t)groups, (uint32_t)std::min<int64_t>(slices, 65535)),
-      dim3(kWriteThreads), args, a.inv_freq ? (size_t)a.per_group * d * sizeof(float) : 0, stream);
+      dim3(kWriteThreads), args, a.inv_freq ? (size_t)a.per_group * d * (sizeof(float) + sizeof(double)) : 0, stream);
   if (e != hipSuccess) return set_error((int)e, "%s launch: %s", what, hipGetErrorString(e));
   return DK_OK;
 }

@@ -538,3 +538,37 @@ def test_decode_bad_page_ids_stay_inside_the_pool():
     for split in (1, 2, 0):
         assert torch.equal(attention.decode_attention(q, cache, tabs[0], bad, tabs[2], split_kv=split),
                            attention.decode_attention(q, cache, tabs[0], zero, tabs[2], split_kv=split))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rotated_codes_are_those_of_the_exact_rotation(dtype, style):
+    """Each code is the one that the rotation in 64 bits rounds to, also beside a boundary between two
+    codes: of 17 million elements an fp32 rotation puts about two on the other side. The 64-bit result
+    is itself off by 2^-52 or so, which reaches a boundary with a chance of 1e-8."""
+    n, hkv, d = 16384, 8, 128
+    g = torch.Generator().manual_seed(11 + style)
+    k = torch.randn(n, hkv, d, generator=g).to(dtype).to(DEV)
+    pos = torch.randint(0, 131072, (n,), generator=g, dtype=torch.int32)
+    pos[:5] = torch.tensor([0, 1, 2, 131071, 0])
+    pos = pos.to(DEV)
+    inv = paging.rope_inv_freq(d, theta=500000.0)
+    cache = layout.alloc_kv4_cache(n // 16, hkv, d, device=DEV)
+    slots = torch.arange(n, device=DEV)
+    paging.write_kv4(k, k, cache, slots, inv_freq=inv, positions=pos, rope_style=style)
+    got = paging.read_kv4(cache, slots)[0].double()
+    angle = pos.double()[:, None] * inv.double()
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    x = k.double()
+    lo, hi = (slice(0, d // 2), slice(d // 2, d)) if style == 0 else (slice(0, d, 2), slice(1, d, 2))
+    y = torch.empty_like(x)
+    y[..., lo] = x[..., lo] * c - x[..., hi] * s
+    y[..., hi] = x[..., hi] * c + x[..., lo] * s
+    b = y.reshape(-1, 32)
+    man, ex = torch.frexp(b.abs().amax(1, keepdim=True))      # man in [1/2, 1)
+    unit = torch.exp2((ex - 3 + (man >= 0.875).to(ex.dtype)).double())
+    z = b / unit
+    step = torch.where(z.abs() < 2, 0.5, torch.where(z.abs() < 4, 1.0, 2.0))
+    want = ((z / step).round() * step * unit).reshape(y.shape)
+    assert int((got != want).sum()) == 0
