@@ -408,7 +408,7 @@ bool short_split_runs(const Problem& p, const Plan& pl, int cus) {
 //  - other lengths: balanced. 100 requests of 100 to 6000 tokens 64.2 against 70.5 in one pass.
 int kv4_auto_split(const Problem& p, const Plan& pl, int cus) {
   const bool windowed = p.opt.window > 0;
-  if (!windowed && p.opt.schedule != 0) return p.opt.schedule == 2;
+  if (!windowed && (p.opt.schedule != 0 || p.opt.waves_per_cu)) return p.opt.schedule == 2;
   const int64_t pairs = (int64_t)p.batch * pl.pairs_per_seq;
   const int64_t hint = p.opt.max_pages_per_seq;
   int64_t pages = hint > 0 ? hint : p.batch == 1 || windowed ? p.num_indices / p.batch : 0;

@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include <algorithm>
+#include <utility>
 #include <string>
 
 namespace dk {
@@ -91,6 +92,15 @@ bool kv4_pool_ok(const void* cache, int64_t num_pages, int64_t kv_p, int32_t hkv
   const __int128 heads = (__int128)(hkv - 1) * kv_h + 17 * head_dim;
   return heads < ((__int128)1 << 31) &&
          ((__int128)std::max<int64_t>(num_pages, 1) - 1) * kv_p + heads < ((__int128)1 << 62);
+}
+
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len) {
+  if (n0 <= 0 || n1 <= 0) return true;
+  if (n1 > 1 && (n0 == 1 || s1 > s0)) {              // n0, s0: the outer one
+    std::swap(n0, n1);
+    std::swap(s0, s1);
+  }
+  return (n1 == 1 || s1 >= len) && (n0 == 1 || s0 >= (__int128)(n1 - 1) * s1 + len);
 }
 
 void partials_layout_rows(int64_t rows, int32_t head_dim, size_t* off_o, size_t* off_m,

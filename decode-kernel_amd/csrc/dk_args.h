@@ -246,6 +246,9 @@ bool pool_ok(int64_t num_pages, const dk_strides& s, int64_t kv_r, int32_t hkv, 
 // of 16 bytes, heads of a page below 2 GiB apart.
 bool kv4_pool_ok(const void* cache, int64_t num_pages, int64_t kv_p, int32_t hkv, int64_t kv_h,
                  int32_t head_dim);
+// Whether the rows of `len` elements at i * s0 + j * s1 (i < n0, j < n1) lie apart, one dimension's
+// strides spanning the other's: what a kernel that writes them needs.
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len);
 int64_t balanced_rows(int32_t batch, int32_t hq, int32_t hkv, int32_t head_dim);
 // Workspace of dk_decode_attention: split 1 -> 0, split > 1 -> explicit partials,
 // split 0 -> balanced partials. 0 on invalid shapes.

@@ -333,6 +333,8 @@ extern "C" int dk_extend_attention_kv4(
   if (!kv4_pool_ok(cache, num_pages, kv_p, num_kv_heads, kv_h, head_dim))
     return set_error(DK_EUNSUPPORTED, "the 4-bit cache must be 16-byte aligned, with page and head "
                                       "strides that are non-negative multiples of 16 bytes");
+  if (!rows_apart(num_tokens, s.o_b, num_q_heads, s.o_h, head_dim))
+    return set_error(DK_EUNSUPPORTED, "the rows of out overlap");
   const int32_t group = num_q_heads / num_kv_heads;
   int64_t first = 0;
   if (const int rc = check_requests(batch, rows, new_lens, all_lens, num_rows, group, num_tokens,

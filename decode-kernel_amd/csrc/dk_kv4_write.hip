@@ -418,6 +418,9 @@ int write_impl(const char* what, void* q, const void* k_new, const void* v_new, 
   if (!kv4_pool_ok(cache, num_pages, s.kv_p, hkv, s.kv_h, d))
     return set_error(DK_EUNSUPPORTED, "the 4-bit cache must be 16-byte aligned, with page and head "
                                       "strides that are non-negative multiples of 16 bytes");
+  if ((q && a.inv_freq && !rows_apart(tokens, s.q_b, hq, s.q_h, d)) ||
+      !rows_apart(num_pages, s.kv_p, hkv, s.kv_h, 17 * d))
+    return set_error(DK_EUNSUPPORTED, "%s: rows of q, or blocks of the cache, overlap", what);
   a.q = static_cast<uint8_t*>(q);
   a.k_new = static_cast<const uint8_t*>(k_new);
   a.v_new = static_cast<const uint8_t*>(v_new);
@@ -515,6 +518,8 @@ extern "C" int dk_kv4_read(const void* cache, int64_t kv_p, int64_t kv_h, const 
   if (!kv4_pool_ok(cache, num_pages, kv_p, num_kv_heads, kv_h, head_dim))
     return set_error(DK_EUNSUPPORTED, "the 4-bit cache must be 16-byte aligned, with page and head "
                                       "strides that are non-negative multiples of 16 bytes");
+  if (!rows_apart(num_tokens, out_t, num_kv_heads, out_h, head_dim))
+    return set_error(DK_EUNSUPPORTED, "dk_kv4_read: the rows of k_out and v_out overlap");
   Kv4ReadArgs a{};
   a.cache = static_cast<const uint8_t*>(cache);
   a.slots = slots;

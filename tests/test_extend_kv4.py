@@ -53,13 +53,14 @@ def test_refusals(kw):
     (dict(q_h=60), dk_lib.DK_EUNSUPPORTED), (dict(kv_p=2200), dk_lib.DK_EUNSUPPORTED),
     (dict(pages=0), dk_lib.DK_EINVAL), (dict(table=None), dk_lib.DK_ENULL), (dict(d=32), dk_lib.DK_EINVAL),
     (dict(scale=0.0), dk_lib.DK_EINVAL), (dict(blocks=9), dk_lib.DK_EINVAL),
+    (dict(o_h=0), dk_lib.DK_EUNSUPPORTED), (dict(o_h=56), dk_lib.DK_EUNSUPPORTED),
     (dict(new=[0], all=[0], q=None), dk_lib.DK_OK)])
 def test_abi_refusals(kw, code):
     a = dict(q=0x10000, cache=0x20000, kv_p=2176, table=0x30000, rows=[1], new=[3], all=[3], d=64, pages=8,
-             q_h=64, scale=0.1, blocks=4)
+             q_h=64, o_h=64, scale=0.1, blocks=4)
     a.update(kw)
     i32 = ctypes.c_int32 * 1
-    s = dk_lib.DkExtendStrides(256, a["q_h"], 0, 0, 0, 0, 256, 64)
+    s = dk_lib.DkExtendStrides(256, a["q_h"], 0, 0, 0, 0, 256, a["o_h"])
     assert dk_lib.load().dk_extend_attention_kv4(
         a["q"], a["cache"], a["kv_p"], 1088, a["table"], 8, 4, a["blocks"], i32(*a["rows"]), i32(*a["new"]),
         i32(*a["all"]), 0x40000, None, 0, 1, 7, 4, 2, a["d"], a["pages"], 0, ctypes.byref(s), a["scale"], 0.0,

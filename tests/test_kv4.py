@@ -572,3 +572,20 @@ def test_rotated_codes_are_those_of_the_exact_rotation(dtype, style):
     step = torch.where(z.abs() < 2, 0.5, torch.where(z.abs() < 4, 1.0, 2.0))
     want = ((z / step).round() * step * unit).reshape(y.shape)
     assert int((got != want).sum()) == 0
+
+
+@pytest.mark.parametrize("q_strides,cache_strides", [
+    ((128, 0), (2176, 1088)), ((64, 64), (2176, 1088)), ((0, 64), (2176, 1088)),
+    ((128, 64), (0, 1088)), ((128, 64), (2176, 1072))])
+def test_write_refuses_rows_that_overlap(q_strides, cache_strides):
+    st = dk_lib.DkStrides(*q_strides, cache_strides[0], 0, 0, cache_strides[1], 0, 0)
+    lib = dk_lib.load()
+    assert lib.dk_kv4_write(0x60000, 0x10000, 0x50000, 128, 64, 0x20000, 0x30000, 0, 0x40000, 0, 0x70000, 0, 3, 2,
+                            2, 64, 4, 0, ctypes.byref(st), None) == dk_lib.DK_EUNSUPPORTED
+    assert b"overlap" in lib.dk_last_error()
+
+
+def test_read_refuses_rows_that_overlap():
+    for out_t, out_h in ((128, 0), (64, 64), (0, 64)):
+        assert dk_lib.load().dk_kv4_read(0x20000, 2176, 1088, 0x30000, 0, 0x40000, 0x50000, out_t, out_h, 3, 2,
+                                         64, 4, 0, None) == dk_lib.DK_EUNSUPPORTED
