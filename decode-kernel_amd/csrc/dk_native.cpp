@@ -16,6 +16,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <vector>
 
 #include "dk_decode.h"
 
@@ -262,18 +263,23 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// ---- paging's calls: block tables, and rows written into and read from a 4-bit cache. Each takes
-// plain calls (no output argument, contiguous vectors, the current device) and returns None for
+// ---- a 4-bit cache's step: block tables, rows written and read, prefill attention. Each takes
+// plain calls (contiguous vectors, the current device, ordinary Python numbers) and returns None for
 // the others, as decode() does; a nonzero C ABI return comes back as an int.
 
 decltype(&dk_grow_block_tables) g_grow = nullptr;
 decltype(&dk_kv4_write) g_kv4_write = nullptr;
 decltype(&dk_kv4_read) g_kv4_read = nullptr;
+decltype(&dk_extend_attention_kv4) g_extend = nullptr;
+decltype(&dk_extend_workspace_bytes) g_extend_bytes = nullptr;
 
-// bind_paging(grow_block_tables, kv4_write, kv4_read: addresses), after bind()
+// bind_paging(grow_block_tables, kv4_write, kv4_read, extend_attention_kv4, extend_workspace_bytes:
+// addresses), after bind()
 PyObject* bind_paging(PyObject*, PyObject* args) {
-  unsigned long long grow, write, read;
-  if (!PyArg_ParseTuple(args, "KKK", &grow, &write, &read)) return nullptr;
+  unsigned long long grow, write, read, extend, bytes;
+  if (!PyArg_ParseTuple(args, "KKKKK", &grow, &write, &read, &extend, &bytes)) return nullptr;
+  g_extend = reinterpret_cast<decltype(g_extend)>(extend);
+  g_extend_bytes = reinterpret_cast<decltype(g_extend_bytes)>(bytes);
   g_grow = reinterpret_cast<decltype(g_grow)>(grow);
   g_kv4_write = reinterpret_cast<decltype(g_kv4_write)>(write);
   g_kv4_read = reinterpret_cast<decltype(g_kv4_read)>(read);
@@ -465,6 +471,91 @@ PyObject* read_impl(PyObject* const* args) {
   return out;
 }
 
+// A list or tuple of n host integers as int32 (n < 0: any number); false: not that
+bool ints_arg(PyObject* o, Py_ssize_t n, std::vector<int32_t>* out) {
+  const bool list = PyList_CheckExact(o);
+  if (!list && !PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t m = list ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
+  if (n >= 0 && m != n) return false;
+  out->resize((size_t)m);
+  for (Py_ssize_t i = 0; i < m; ++i)
+    if (!int_arg(list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i), &(*out)[i])) return false;
+  return true;
+}
+
+// (q, cache, block_table, rows, new_lens, all_lens, out, scale, logit_cap, window, sinks): the output
+PyObject* extend_impl(PyObject* const* args) {
+  const at::Tensor *q = tensor_arg(args[0]), *c = tensor_arg(args[1]), *t = tensor_arg(args[2]);
+  const int64_t d = cache_dim(c);
+  if (!q || !t || !d) Py_RETURN_NONE;
+  const at::Device dev = c->device();
+  const bool f16 = q->scalar_type() == at::kHalf;
+  if (!(f16 || q->scalar_type() == at::kBFloat16) || q->dim() != 3 || q->device() != dev ||
+      q->size(2) != d || q->stride(2) != 1 || q->size(1) <= 0 || q->size(1) % c->size(1) ||
+      q->size(1) > INT32_MAX || t->scalar_type() != at::kInt || t->dim() != 2 || t->device() != dev ||
+      (t->stride(1) != 1 && t->size(1) > 1) || t->size(1) > INT32_MAX)
+    Py_RETURN_NONE;
+  std::vector<int32_t> rows, news, alls;
+  if (!ints_arg(args[3], -1, &rows) || !ints_arg(args[4], (Py_ssize_t)rows.size(), &news) ||
+      !ints_arg(args[5], (Py_ssize_t)rows.size(), &alls) || rows.size() > INT32_MAX)
+    Py_RETURN_NONE;
+  at::Tensor out;
+  if (args[6] != Py_None) {
+    const at::Tensor* o = tensor_arg(args[6]);
+    if (!o || o->sizes() != q->sizes() || o->scalar_type() != q->scalar_type() ||
+        o->device() != dev || o->stride(2) != 1)
+      Py_RETURN_NONE;
+    out = *o;
+  }
+  bool given = false;
+  float scale = 0.f, cap = 0.f;
+  int32_t window = 0;
+  const bool no_cap = PyFloat_CheckExact(args[8]) && PyFloat_AS_DOUBLE(args[8]) == 0.0;
+  if (!positive_arg(args[7], &given, &scale)) Py_RETURN_NONE;
+  if (!given) scale = (float)(1.0 / std::sqrt((double)d));
+  if ((!no_cap && !positive_arg(args[8], &given, &cap)) ||
+      (args[9] != Py_None && !int_arg(args[9], &window)))
+    Py_RETURN_NONE;
+  const float* sinks = nullptr;
+  if (args[10] != Py_None) {
+    const at::Tensor* x = tensor_arg(args[10]);
+    if (!x || x->scalar_type() != at::kFloat || x->dim() != 1 || x->size(0) != q->size(1) ||
+        !x->is_contiguous() || x->device() != dev)
+      Py_RETURN_NONE;
+    sinks = static_cast<const float*>(x->data_ptr());
+  }
+  void* raw = nullptr;
+  const int on = stream_of(dev, &raw);
+  if (on < 0) return nullptr;
+  if (!on) Py_RETURN_NONE;
+  const int32_t n = (int32_t)rows.size(), hq = (int32_t)q->size(1), hkv = (int32_t)c->size(1);
+  const size_t need = g_extend_bytes(n, news.data(), alls.data(), hq, hkv, (int32_t)d, window);
+  if (!out.defined()) out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor ws;
+  if (need) ws = at::empty({(int64_t)need}, c->options());
+  dk_extend_strides s{};
+  s.q_b = q->stride(0);
+  s.q_h = q->stride(1);
+  s.o_b = out.stride(0);
+  s.o_h = out.stride(1);
+  const void *qd = q->data_ptr(), *cd = c->data_ptr();
+  void *od = out.data_ptr(), *wd = need ? ws.data_ptr() : nullptr;
+  const int32_t* td = static_cast<const int32_t*>(t->data_ptr());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_extend(qd, cd, c->stride(0), c->stride(1), td, t->stride(0), t->size(0),
+                (int32_t)t->size(1), rows.data(), news.data(), alls.data(), od, wd, need, n,
+                q->size(0), hq, hkv, (int32_t)d, c->size(0), f16 ? DK_F16 : DK_BF16, &s, scale, cap,
+                window, sinks, raw);
+  Py_END_ALLOW_THREADS
+  if (rc != DK_OK) return PyLong_FromLong(rc);
+  if (args[6] != Py_None) {
+    Py_INCREF(args[6]);
+    return args[6];
+  }
+  return THPVariable_Wrap(std::move(out));
+}
+
 template <PyObject* (*Impl)(PyObject* const*), int N>
 PyObject* paging_call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != N || !g_grow || !g_get_device) {
@@ -496,6 +587,8 @@ PyMethodDef kMethods[] = {
      "write_kv4's arguments: the C ABI's return, or None"},
     {"read_kv4", fast_call<read_impl, 3>(), METH_FASTCALL,
      "cache, slots, dtype code: (k, v), a C ABI error code, or None"},
+    {"extend_attention_kv4", fast_call<extend_impl, 11>(), METH_FASTCALL,
+     "extend_attention_kv4's arguments: the output, a C ABI error code, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dk_native", nullptr, -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -150,6 +150,14 @@ def extend_attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torc
 
     A page id outside the cache gives NaN to the tokens that attend to it. Returns out."""
     what = "extend_attention_kv4"
+    native = paging._NATIVE or paging._native()
+    if native:
+        got = native.extend_attention_kv4(q, cache, block_table, rows, new_lens, all_lens, out, scale,
+                                          logit_cap, window, sinks)
+        if isinstance(got, torch.Tensor):
+            return got
+        if got is not None:
+            dk_lib.check(got, what)
     for name, t in (("q", q), ("cache", cache), ("block_table", block_table)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")

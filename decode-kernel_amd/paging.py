@@ -119,19 +119,21 @@ _NATIVE = None   # _dk_native once bound to the loaded library; False where it i
 
 
 def _native():
-    """_dk_native with paging's calls bound, or False (csrc/dk_native.cpp). It takes the plain calls
-    of a step, each at about the cost of its launch: grow_block_tables costs 4.7 us on the host
-    against 13.1 in Python, write_kv4 3.1 against 11.1, read_kv4 3.8 against 8.9."""
+    """_dk_native with the calls of a 4-bit cache's step bound, or False (csrc/dk_native.cpp). It takes
+    the plain ones, each at about the cost of its launch: grow_block_tables costs 4.7 us on the host
+    against 13.1 in Python, write_kv4 3.1 against 11.1, read_kv4 3.8 against 8.9,
+    extend.extend_attention_kv4 5.5 against 15.2."""
     global _NATIVE
     if _NATIVE is None:
         import attention
         decode = attention._bind_native()
         module = sys.modules.get("_dk_native")
         if module is not None and getattr(module, "decode", None) is decode and \
-                hasattr(module, "bind_paging"):
+                hasattr(module, "extend_attention_kv4"):
             lib = dk_lib.load()
             module.bind_paging(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
-                lib.dk_grow_block_tables, lib.dk_kv4_write, lib.dk_kv4_read)))
+                lib.dk_grow_block_tables, lib.dk_kv4_write, lib.dk_kv4_read,
+                lib.dk_extend_attention_kv4, lib.dk_extend_workspace_bytes)))
             _NATIVE = module
         else:
             _NATIVE = False

@@ -8,6 +8,7 @@ import torch
 
 import _dk_native
 import attention
+import extend
 import layout
 import paging
 from dk_lib import DecodeArgumentError
@@ -80,6 +81,50 @@ def test_rows_are_the_same(python_path, dtype, rope, i64):
         assert torch.equal(x, y)
 
 
+def _prefill(dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(5)
+    cache = layout.alloc_kv4_cache(60, 2, 64, device="cuda")
+    k = torch.randn(960, 2, 64, generator=g).to(dtype).cuda()
+    paging.write_kv4(k, k.flip(0), cache, torch.arange(960, device="cuda"))
+    table = torch.arange(60, dtype=torch.int32, device="cuda").view(1, 60).repeat(3, 1)
+    return torch.randn(80, 6, 64, generator=g).to(dtype).cuda(), cache, table
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prefill_is_the_same(python_path, dtype):
+    q, cache, table = _prefill(dtype)
+    sinks = torch.randn(6, device="cuda")
+    for kw in (dict(), dict(scale=0.3), dict(logit_cap=0.0, window=0), dict(logit_cap=9.0, window=50, sinks=sinks),
+               dict(out=torch.empty(80, 6, 64, dtype=dtype, device="cuda")),
+               dict(out=torch.empty(6, 80, 64, dtype=dtype, device="cuda").transpose(0, 1))):
+        for args in (([0, 2], [30, 50], [33, 700]), ((1,), (3,), (960,)), ([], [], [])):
+            got = extend.extend_attention_kv4(q, cache, table, *args, **kw)
+            assert got is kw["out"] if "out" in kw else got.is_contiguous()
+            mine = got.clone()
+            want = python_path(lambda: extend.extend_attention_kv4(q, cache, table, *args, **kw))
+            n = sum(args[1])
+            assert torch.equal(mine[:n], want[:n]), (kw, args)
+
+
+@pytest.mark.gpu
+def test_the_module_takes_plain_prefill_calls():
+    q, cache, table = _prefill()
+    call = (q, cache, table, [0, 2], [30, 50], [33, 700], None, None, None, None, None)
+    native = paging._native()
+    assert isinstance(native.extend_attention_kv4(*call), torch.Tensor)
+    assert native.extend_attention_kv4(*call[:4], [30, 51], *call[5:]) not in (0, None)      # more than q has
+    for at, bad in ((0, q.float()), (0, q[..., :32]), (0, q[:, :5]), (1, cache.cpu()), (2, table.long()),
+                    (3, [0]), (3, [0, -1]), (3, torch.tensor([0, 2])), (4, [30, 50.0]), (5, [33, 2 ** 40]),
+                    (6, torch.empty_like(q).float()), (7, 1), (7, -1.0), (8, -2.0), (9, -3), (9, 2.0),
+                    (10, torch.zeros(5, device="cuda"))):
+        assert native.extend_attention_kv4(*call[:at], bad, *call[at + 1:]) is None, (at, bad)
+    with pytest.raises(DecodeArgumentError):
+        extend.extend_attention_kv4(q, cache, table, [0, 2], [30, 51], [33, 700])
+    got = extend.extend_attention_kv4(q, cache, table, torch.tensor([0, 2]), [30, 50], [33, 700])
+    assert torch.equal(got[:80], native.extend_attention_kv4(*call)[:80])
+
+
 @pytest.mark.gpu
 def test_the_module_takes_the_plain_calls():
     native = paging._native()
@@ -128,7 +173,8 @@ def test_left_to_python_without_a_gpu():
     assert native.read_kv4(cache, slots, 0) is None
     assert native.grow_block_tables(*(None,) * 7) is None
     assert native.write_kv4(*(None,) * 8) is None and native.read_kv4(*(None,) * 3) is None
-    for fn in (native.grow_block_tables, native.write_kv4, native.read_kv4):
+    assert native.extend_attention_kv4(*(None,) * 11) is None
+    for fn in (native.grow_block_tables, native.write_kv4, native.read_kv4, native.extend_attention_kv4):
         with pytest.raises(TypeError):
             fn(k)
 
