@@ -10,15 +10,15 @@
 //   * LDS rows are padded rather than swizzled: 16 rows' 16-byte chunks (K) and 4 rows' 64-byte runs
 //     (V, transpose reads) lie in different banks, and every address is a base and a constant;
 //   * a weight enters as two parts of q's type: 22 bits in fp16 (ExtendParts<F16>), in bf16 16, off by
-//     2^-18 of itself where the output's own rounding is 2^-9 (a third part adds 1e-6 of the norm and
-//     costs 12 %).
+//     at most 2^-16 of itself where the output's own rounding is 2^-8 (a third part takes 1e-6 off the
+//     error of the norm and costs 12 %).
 // Bound by the card's power where a call is long: q.k and both parts of p run at 1,120 TFLOP/s, where
 // a large library product ends at 1,305 to 1,360, and a variant with a third less MFMA work is only 16 %
 // faster, one without exponentials 7 %. 32/8/128, 2048 new of 8192 tokens, us: fp16 323, bf16 318 (dk_extend
 // over 16-bit rows 376, 441); one workgroup loop of MFMA phase, softmax, staging in turn 348, 336. 8
 // requests of 79-730 new tokens over up to 500 (32/8/64 bf16) 38.6: bound by the VALU, 1.0 us per
 // workgroup and 64-key tile on a CU that holds three, and by the longest workgroup, 16 tiles of
-// 1.75 us. Tiles dealt to the workgroups that the chip holds (ExtendKv4Args) against one workgroup
+// 1.75 us each. Tiles dealt to the workgroups that the chip holds (ExtendKv4Args) against one workgroup
 // per tile: 38.6 and 42.6, one request of 2048 tokens (32/8/128 fp16) 65.3 and 67.8.
 #pragma once
 

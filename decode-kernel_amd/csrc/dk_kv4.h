@@ -102,6 +102,12 @@ __device__ __forceinline__ constexpr int q_part_exp(int i) { return 1 + 5 * i; }
 //     dims has p in the even k and 0 in the odd ones. The 16 rows are 4 heads x (parity, part).
 //     HP = 8, 16: k = tokens of two pages, the pairs regrouped by token (v_perm); rows are the heads,
 //     and for HP = 8 the parts share an MFMA, each page's lo in the rows of the other page.
+// Bound by HBM reads at D = 128 and 256 with up to 4 heads: 32 x 8192 tokens of 32/8/128 fp16 48 us (286
+// MB; 6.5 TB/s between start and end, where reads of this page pattern without arithmetic reach 6.8). At
+// D = 64, whose pages hold half the bytes per instruction, by instruction issue (79 % of the cycles): 128
+// x 128..8192 tokens of 64/8/64 bf16 65 us and a merge (292 MB, 4.5 TB/s; the pattern 6.2); three
+// wavefronts per SIMD instead of two 73 against 71. With 8 and 16 heads by the matrix instructions'
+// dependent chains: 16 x 32768 of 64/8/128 fp16 94 us, 8 x 65536 of 128/8/128 bf16 97 (6.1 and 5.9 TB/s).
 template <class T, int D, int HP, bool CAP>
 struct Kv4Wave {
   static constexpr int kStep = D <= 128 ? 4 : 2;   // pages per step

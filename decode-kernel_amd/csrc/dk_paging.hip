@@ -214,8 +214,8 @@ __device__ __forceinline__ GrowRequest grow_request(const GrowArgs& a, int b) {
 // outputs are sums over the requests before it, recomputed per workgroup as dk_page_table does:
 // the blocks (kv_indices), the blocks that are new (the ids handed out), the new tokens. A new
 // block's id comes straight from `pages`, so no workgroup reads what another writes (requests
-// name different rows). One launch in place of some 30 small ones, bound by its latency (lengths,
-// rows and table, three dependent reads).
+// name different rows). One launch in place of some 30 small ones (380 us), bound by its latency
+// (lengths, rows and table, three dependent reads): 32 requests of up to 8192 tokens 4.2 us, 500 4.9.
 __global__ __launch_bounds__(kThreads) void dk_grow_tables(GrowArgs a) {
   __shared__ int64_t partial[3][kThreads / 64];
   const int b = blockIdx.x;

@@ -3,9 +3,10 @@ and decode attention over it, against the float64 oracle (oracle/kv4.py).
 
 Tolerances. Stored values are compared exactly where nothing is computed (V, unrotated K); a rotated
 element may take the neighbouring code where its exact value lies within fp32's error of the border
-between them. Attention: scores are sums of exact products with what the MFMA's 13-bit window and fp32
-drop, at most 2^-14 of sum |q_i k_i| * scale (at most 15 addends of a group lose 2^-18 of its largest
-product each); a weight is off by that, by the 2^-16 of its two bf16 parts and by fp32; so an output moves
+between them (float64's since the rotation is in double: the last test). Attention: scores are exact
+sums over q's E2M3 parts, which hold elements down to 2^-7 (bf16) or 2^-9 (fp16) of their block's largest
+whole and cut smaller ones by at most 2^-15 of it; for the normal rows here, where one element in 60 is
+that small, and with fp32's sums over a row, that is below 2^-14 of sum |q_i k_i| * scale; a weight is off by that, by the 2^-16 of its two bf16 parts and by fp32; so an output moves
 by at most twice the weights' error times (max |v| + |out|), and is rounded once, by half a step of its
 type."""
 import ctypes
