@@ -199,7 +199,7 @@ def grow_block_tables(block_table: torch.Tensor, rows: torch.Tensor, cached_lens
         got = native.grow_block_tables(block_table, rows, cached_lens, new_lens, new_pages,
                                        num_tokens, capacity)
         if type(got) is tuple:
-            return StepTables._make(got)
+            return tuple.__new__(StepTables, got)
         if got is not None:
             dk_lib.check(got, what)
     for name, t in (("block_table", block_table), ("new_pages", new_pages)):
