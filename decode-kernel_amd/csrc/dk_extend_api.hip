@@ -365,8 +365,8 @@ extern "C" int dk_extend_attention_kv4(
   a.num_slots = (uint32_t)num_pages;
   const bool bf16 = dtype == DK_BF16, cap = logit_cap != 0.f;
   const float stage = (float)(1 << (bf16 ? kv4_stage_exp<BF16>() : kv4_stage_exp<F16>()));
-  a.kscale = kLog2e * score_scale * stage;
-  a.cap_in = cap ? score_scale * stage / logit_cap : 0.f;
+  a.kscale = kLog2e * score_scale;
+  a.cap_in = cap ? score_scale / logit_cap : 0.f;
   a.cap_out = kLog2e * logit_cap;
   a.vscale = stage;
   const void* fn = head_dim == 64    ? extend_kv4_symbol<64>(bf16, cap)

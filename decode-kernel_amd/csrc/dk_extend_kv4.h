@@ -2,24 +2,26 @@
 //
 // dk_extend.h's mathematics (S^T = K.Q^T, O^T += V^T.P^T, 128 query rows of one kv head per workgroup,
 // 32 per wavefront), over page blocks found through a block table:
-//   * a wavefront loads a page's 17 D bytes a tile ahead (a quarter of 16-bit rows' traffic) and
-//     widens them to q's type on the way into LDS, in pieces between the last P.V products of the
-//     tile before, whose MFMAs leave the VALU free;
-//   * a tile's A operands are read from LDS four steps ahead of the MFMA that takes them, and its
+//   * q.k on v_mfma_scale_f32_32x32x64_f8f6f4, at four times the rate of 16-bit operands: K's codes and
+//     scales as they lie in the page, q as 3 parts of E2M3 with scales of their own, so three quarters
+//     of the 16-bit time, a quarter of the LDS traffic and no widening (2048 new of 8192 tokens, fp16
+//     322 -> 298 us; with K widened to q's type);
+//   * V is widened to q's type on its way into LDS, in pieces between the last P.V products of the tile
+//     before, whose MFMAs leave the VALU free; a wavefront loads a page's 17 D bytes a tile ahead;
+//   * a tile's A operands are read from LDS several steps ahead of the MFMA that takes them, and its
 //     two 32-key blocks are staggered: the second's weights are formed beside the first's products;
 //   * LDS rows are padded rather than swizzled: 16 rows' 16-byte chunks (K) and 4 rows' 64-byte runs
 //     (V, transpose reads) lie in different banks, and every address is a base and a constant;
 //   * a weight enters as two parts of q's type: 22 bits in fp16 (ExtendParts<F16>), in bf16 16, off by
 //     at most 2^-16 of itself where the output's own rounding is 2^-8 (a third part takes 1e-6 off the
 //     error of the norm and costs 12 %).
-// Bound by the card's power where a call is long: q.k and both parts of p run at 1,120 TFLOP/s, where
-// a large library product ends at 1,305 to 1,360, and a variant with a third less MFMA work is only 16 %
-// faster, one without exponentials 7 %. 32/8/128, 2048 new of 8192 tokens, us: fp16 323, bf16 318 (dk_extend
-// over 16-bit rows 376, 441); one workgroup loop of MFMA phase, softmax, staging in turn 348, 336. 8
-// requests of 79-730 new tokens over up to 500 (32/8/64 bf16) 38.6: bound by the VALU, 1.0 us per
-// workgroup and 64-key tile on a CU that holds three, and by the longest workgroup, 16 tiles of
-// 1.75 us each. Tiles dealt to the workgroups that the chip holds (ExtendKv4Args) against one workgroup
-// per tile: 38.6 and 42.6, one request of 2048 tokens (32/8/128 fp16) 65.3 and 67.8.
+// Bound by the card's power where a call is long: the clock settles at 1.6 to 2.0 GHz, and a variant
+// with a third less MFMA work was only 16 % faster, one without exponentials 7 %. 32/8/128, 2048 new of
+// 8192 tokens, us: fp16 298, bf16 291 (dk_extend over 16-bit rows 376, 441). 8 requests of 79-730 new
+// tokens over up to 500 (32/8/64 bf16) 37.8: bound by the VALU, 1.0 us per workgroup and 64-key tile on a
+// CU that holds three, and by the longest workgroup, 16 tiles of 1.75 us each. Tiles dealt to the
+// workgroups that the chip holds (ExtendKv4Args) against one workgroup per tile: 38.6 and 42.6 there,
+// one request of 2048 tokens (32/8/128 fp16) 65.3 and 67.8.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,6 +33,12 @@
 namespace dk {
 
 constexpr int kKv4ExtendOrder = 256;  // query tiles that a call deals out itself (ExtendKv4Args)
+
+// E2M3 parts of q (QParts): what 3 leave of an element is at most 2^-15 of the power of two below its 32
+// dims' largest magnitude. bf16 is whole down to 2^-7 of that, fp16 down to 2^-4, and what smaller
+// elements lose is a sixteenth of the largest one's own rounding. A fourth part for fp16 (as in decode,
+// which waits for memory) costs 4.5 %: 312 us against 298 for 2048 new of 8192 tokens.
+constexpr int kKv4ExtendQParts = 3;
 
 // Workgroups that a CU holds at once
 constexpr int kv4_extend_resident(int d, bool cap) { return d == 64 ? (cap ? 2 : 3) : d == 128 ? 2 : 1; }
@@ -45,8 +53,8 @@ struct ExtendKv4Args {
   uint16_t list[kKv4ExtendOrder], start[kKv4ExtendOrder + 1];
 };
 
-// Rows are staged in q's type, in fp16 at half their size (exact, the factor returned by the score
-// scale and the output's): E2M1's 6 times the largest scale of an fp16 value, 4 * 2^14, is past
+// V is staged in q's type, in fp16 at half its size (exact, the factor returned by the output's
+// scale): E2M1's 6 times the largest scale of an fp16 value, 4 * 2^14, is past
 // fp16's range.
 template <class T>
 constexpr int kv4_stage_exp() { return __is_same(T, F16) ? 1 : 0; }
@@ -88,6 +96,57 @@ __device__ __forceinline__ float less(BF16, float x, u32 pair) {
   return BF16::dot2(pair, minus, x);
 }
 
+// C += A.B: A 32 keys x 64 dims of E2M1, B 64 dims x 32 rows of E2M3; lane half h holds dims 32 h .. of
+// both. Byte GA of sa / GB of sb: the E8M0 scale of the lane's key / row for those 32.
+template <int GA, int GB>
+__device__ __forceinline__ f32x16 mfma_mx32(u32x4 a, u32x6 b, f32x16 c, u32 sa, u32 sb) {
+  const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], (int)b[4], (int)b[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 2, GA, (int)sa, GB, (int)sb);
+}
+
+// 32 values of q (16 words) as QP parts of E2M3 and their scales' bytes (QParts; a block with a NaN
+// or an infinity gets the NaN scale)
+template <class T, int QP>
+__device__ __forceinline__ void q_parts(const u32 (&w)[16], u32x6 (&part)[QP], u32* scales) {
+  f32x16v lo, hi;                                // even and odd dims
+  u32 top = 0u;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float x, y;
+    if constexpr (__is_same(T, F16)) {
+      const f16x2 v = __builtin_bit_cast(f16x2, w[i]);
+      x = (float)v[0];
+      y = (float)v[1];
+    } else {
+      x = __builtin_bit_cast(float, w[i] << 16);
+      y = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+    }
+    lo[i] = x;
+    hi[i] = y;
+    top = max(top, max(__builtin_bit_cast(u32, x) & 0x7fffffffu, __builtin_bit_cast(u32, y) & 0x7fffffffu));
+  }
+  const int ex = top == 0u ? 127 : max((int)(top >> 23), q_part_exp(QP - 1) + 1);
+  *scales = 0u;
+  for_each<QP>([&](auto ic) {
+    constexpr int i = ic.value;
+    const float sc = __builtin_bit_cast(float, (u32)(min(ex, 254) - q_part_exp(i)) << 23);
+    const u32x6 q6 = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(lo, hi, sc);
+    asm volatile("" ::"v"(lo), "v"(hi), "v"(sc), "v"(q6));   // no shared register (Kv4Wave::load_q)
+    part[i] = q6;
+    *scales |= (u32)(ex == 255 ? 255 : ex - q_part_exp(i)) << (8 * i);
+    if constexpr (i + 1 < QP) {
+      const f32x32v back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q6, sc);
+      asm volatile("" ::"v"(q6), "v"(sc), "v"(back));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        lo[j] -= back[2 * j];
+        hi[j] -= back[2 * j + 1];
+      }
+    }
+  });
+}
+
 template <class T, int D, bool CAP>
 __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void dk_extend_kv4(ExtendKv4Args ka) {
   const ExtendArgs& a = ka.e;
@@ -95,11 +154,14 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
   constexpr int BN = 32 * NB;
   // Bytes per LDS row, padded so that 16 rows' chunks of 16 bytes (K) and 4 rows' runs of 64 (V) fall
   // into different banks: every offset is then a constant of the instruction
-  constexpr int KB = 2 * D + 16, VB = 2 * D + 64;
-  constexpr int KT = BN * KB, BUF = KT + BN * VB;  // K's tile, both
   constexpr int DB = D / 32;                      // 32-dim blocks
-  constexpr int QK = D / 16;                      // q.k MFMAs per 32-key block
-  constexpr int kAhead = 4;
+  constexpr int KB = D / 2 + 16, VB = 2 * D + 64;
+  constexpr int KS = BN * KB, KT = KS + BN * DB;   // K's scales (DB bytes per key), V's tile
+  constexpr int BUF = KT + BN * VB;
+  constexpr int KM = D / 64;                      // 64-dim parts of a row
+  constexpr int QP = kKv4ExtendQParts;
+  constexpr int PV = D / 16;                      // steps of a 32-key block's V: 16 keys x 32 dims
+  constexpr int kAhead = D > 64 ? 4 : __is_same(T, BF16) ? 3 : 2;   // what the registers hold
   constexpr int WP = D == 256 ? 2 : 1;            // wavefronts that stage a page, 128 dims (64) each
   constexpr int BW = D == 64 ? 2 : 4;             // words of a lane's K codes and V codes
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUF];
@@ -155,12 +217,25 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
     kend = min(kbeg + per, kend);
   }
 
-  u32x4 qf[QK];
+  // q as E2M3 parts (QParts), lane (h, c): dims 64 m + 32 h .. of row c
+  u32x6 qf[KM][QP];
+  u32 qs[KM];                          // their scales, a byte each
   {
     const uint8_t* qp = a.q + (int64_t)(rq.q0 + rr / G) * a.q_b +
-                        (int64_t)(kvh * G + rr % G) * a.q_h + 16 * h;
+                        (int64_t)(kvh * G + rr % G) * a.q_h + 64 * h;
 #pragma unroll
-    for (int i = 0; i < QK; ++i) qf[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+    for (int m = 0; m < KM; ++m) {
+      u32 words[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 128 * m + 16 * i);
+        words[4 * i] = x[0];
+        words[4 * i + 1] = x[1];
+        words[4 * i + 2] = x[2];
+        words[4 * i + 3] = x[3];
+      }
+      q_parts<T, QP>(words, qf[m], &qs[m]);
+    }
   }
 
   // ---- loads: wavefront w takes page pg of the tile, part sp of its dims. Lane (sr, st): block sr
@@ -221,19 +296,22 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
     }
     if (__builtin_amdgcn_ballot_w64(found)) nan_tile[buf != 0][w] = (u32)j + 1u;
   };
-  // Staging, in pieces of a chunk or row: K's BW chunks of 8 dims, then V's 4 tokens
-  constexpr int PIECES = BW + 4;
-  uint8_t* const kput = smem + (pg * kPage + st) * KB + 256 * sp + 16 * BW * sr;
+  // Staging, in pieces: K's codes and scale as they are, V's 4 tokens
+  constexpr int PIECES = 5;
+  uint8_t* const kput = smem + (pg * kPage + st) * KB + 64 * sp + 4 * BW * sr;
+  uint8_t* const ksput = smem + KS + (pg * kPage + st) * DB + (D == 64 ? sr / 2 : 4 * sp + sr);
   uint8_t* const vput = smem + KT + (pg * kPage + 4 * sr) * VB + 256 * sp + (D == 64 ? 8 : 16) * st;
   auto store_piece = [&](auto piece, int buf) {
     constexpr int p = decltype(piece)::value;
-    if constexpr (p < BW) {
-      const u32 sc = kv4_stage_scale<T>(ksc << 23);
-      *reinterpret_cast<u32x4*>(kput + buf + 16 * p) =
-          u32x4{from_fp4<T, 0>(kr[p], sc), from_fp4<T, 1>(kr[p], sc), from_fp4<T, 2>(kr[p], sc),
-                from_fp4<T, 3>(kr[p], sc)};
+    if constexpr (p == 0) {
+      typedef u32 Run __attribute__((ext_vector_type(BW)));
+      Run x;
+#pragma unroll
+      for (int i = 0; i < BW; ++i) x[i] = kr[i];
+      *reinterpret_cast<Run*>(kput + buf) = x;
+      ksput[buf] = (uint8_t)ksc;
     } else {
-      constexpr int x = p - BW;
+      constexpr int x = p - 1;
       const u32 sc = kv4_stage_scale<T>(e8m0_exp<x>(vsc));
       if constexpr (D == 64) {
         const u32 v = vr[x / 2] >> (16 * (x & 1));
@@ -260,12 +338,23 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
 
   // this lane's places in the tiles it reads (dk_extend.h)
   const uint8_t* const kget = smem + c * KB + 16 * h;
+  const uint8_t* const ksget = smem + KS + c * DB;
   const uint8_t* const vget = smem + KT + (4 * h + ((lane & 15) >> 2)) * VB +
                               32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
-  // A operands: 16 dims (step i) of block n's keys; 16 keys' 32 dims (step y of 2 * DB) of its V
-  auto read_k = [&](int n, int i, int buf) {
-    return *reinterpret_cast<const u32x4*>(kget + buf + 32 * n * KB + 32 * i);
+  // A operands: 64 dims (part m) of block n's keys, and their scales (byte 0: 64 m + 32 h .. of an even
+  // m, byte 2 of an odd one); 16 keys' 32 dims (step y of PV) of its V
+  auto read_k = [&](int n, int m, int buf) {
+    return *reinterpret_cast<const u32x4*>(kget + buf + 32 * n * KB + 32 * m);
+  };
+  auto read_ks = [&](int n, int buf, u32 (&sc)[(KM + 1) / 2]) {
+    const uint8_t* p = ksget + buf + 32 * n * DB;
+    if constexpr (D == 64) {
+      sc[0] = (u32)*reinterpret_cast<const uint16_t*>(p) >> (8 * h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KM / 2; ++i) sc[i] = reinterpret_cast<const u32*>(p)[i] >> (8 * h);
+    }
   };
   auto read_v = [&](int n, int y, int buf) {
     const uint8_t* vp = vget + buf + (32 * n + 16 * (y / DB)) * VB + 64 * (y % DB);
@@ -375,20 +464,27 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
       float mx;
       // the tile's A operands, read kAhead steps before their use: all keys, then all values
       u32x4 ahead[kAhead];
+      u32 ks0[(KM + 1) / 2], ks1[(KM + 1) / 2];
       auto fetch = [&](int g) {
-        if (g < 2 * NB * QK)
-          ahead[g % kAhead] = g < NB * QK ? read_k(g / QK, g % QK, buf)
-                                          : read_v(g / QK - NB, g % QK, buf);
+        if (g < NB * (KM + PV))
+          ahead[g % kAhead] = g < NB * KM ? read_k(g / KM, g % KM, buf)
+                                          : read_v((g - NB * KM) / PV, (g - NB * KM) % PV, buf);
       };
+      read_ks(0, buf, ks0);
+      if constexpr (NB == 2) read_ks(1, buf, ks1);
 #pragma unroll
       for (int g = 0; g < kAhead; ++g) fetch(g);
-#pragma unroll
-      for (int i = 0; i < NB * QK; ++i) {
-        f32x16& x = i < QK ? s0 : s1;
-        x = mfma32(T{}, ahead[i % kAhead], qf[i % QK], i % QK ? x : f32x16{});
-        fetch(i + kAhead);
+      for_each<NB * KM>([&](auto g) {
+        constexpr int n = g.value / KM, m = g.value % KM;
+        f32x16& x = n ? s1 : s0;
+        const u32 sc = n ? ks1[m / 2] : ks0[m / 2];
+        for_each<QP>([&](auto i) {
+          x = mfma_mx32<2 * (m % 2), i.value>(ahead[g.value % kAhead], qf[m][i.value],
+                                              m || i.value ? x : f32x16{}, sc, qs[m]);
+        });
+        fetch(g.value + kAhead);
         pin();
-      }
+      });
       mask(j * BN, s0, nan_pages, buf);
       mx = top_of(s0);
       if constexpr (NB == 2) {
@@ -402,9 +498,9 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
         // the first block's V products beside the second's weights
         for_each<8>([&](auto x) {
 #pragma unroll
-          for (int y = x.value * QK / 8; y < (x.value + 1) * QK / 8; ++y) {
-            pv(y, ahead[(2 * QK + y) % kAhead], p0);
-            fetch(2 * QK + y + kAhead);
+          for (int y = x.value * PV / 8; y < (x.value + 1) * PV / 8; ++y) {
+            pv(y, ahead[(NB * KM + y) % kAhead], p0);
+            fetch(NB * KM + y + kAhead);
           }
           weigh(x.value, s1, p1);
           pin();
@@ -413,9 +509,9 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
       // the last block's V products beside the staging of the next tile
       fix();
       for_each<PIECES>([&](auto p) {
-        constexpr int at = (2 * NB - 1) * QK;
+        constexpr int at = NB * KM + (NB - 1) * PV;
 #pragma unroll
-        for (int y = p.value * QK / PIECES; y < (p.value + 1) * QK / PIECES; ++y) {
+        for (int y = p.value * PV / PIECES; y < (p.value + 1) * PV / PIECES; ++y) {
           pv(y, ahead[(at + y) % kAhead], NB == 2 ? p1 : p0);
           fetch(at + y + kAhead);
         }
