@@ -32,6 +32,41 @@ int extend_split(int32_t batch, const int32_t* new_lens, const int32_t* all_lens
   return (int)std::min<int64_t>(std::max<int64_t>(s, 1), kExtendMaxSplit);
 }
 
+// The same over a 4-bit cache: of the splits up to that one, the one with the least time, its parts
+// being the longest query tile's keys (kKv4TileCost per 64 of them, more where two workgroups share a
+// CU) and, split, the partials' way through memory and the merge's launch. us, this choice and the one
+// above: one request of 512 tokens (32/8/128 fp16) 19.7 and 27.8, of 1024 33.3 and 52.1, (32/8/64)
+// 24.6 and 34.7; 64 new of 4064 22.5 both, in one part 99.6; 512 of 2512 51.7 both, in one part 68.3.
+int extend_split_kv4(int32_t batch, const int32_t* new_lens, const int32_t* all_lens, int32_t hkv,
+                     int32_t group, int32_t head_dim, int32_t window) {
+  const int most = extend_split(batch, new_lens, all_lens, hkv, group, window);
+  if (most == 1) return 1;
+  const double per_tile = head_dim == 64 ? 1.6 : head_dim == 128 ? 2.1 : 4.6;   // us per 64 keys
+  const double shared = head_dim == 256 ? 2.0 : 1.5;   // where two workgroups take turns on a CU
+  constexpr double kMerge = 4.5, kPartials = 4.0e6;    // us; bytes per us
+  int64_t groups = 0, keys = 0, tokens = 0;
+  for (int32_t b = 0; b < batch; ++b) {
+    if (new_lens[b] <= 0) continue;
+    groups += ((int64_t)new_lens[b] * group + kExtendRows - 1) / kExtendRows * hkv;
+    const int64_t seen = window > 0 ? (int64_t)window + kExtendRows / group + 1 : INT32_MAX;
+    keys = std::max<int64_t>(keys, std::min<int64_t>(all_lens[b], seen));
+    tokens += new_lens[b];
+  }
+  const double tiles = (double)((keys + 63) / 64);
+  const double part = (double)tokens * hkv * group * head_dim * 2 * sizeof(float) / kPartials;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= most; ++s) {
+    const double turns = groups * s > kExtendFill / 2 ? shared : 1.0;
+    const double cost = std::ceil(tiles / s) * per_tile * turns + (s > 1 ? kMerge + part * s : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 template <class T>
 hipError_t merge(const ExtendArgs& a, int64_t tokens, int d, bool keep_nan, hipStream_t stream) {
   MergeArgs m{};
@@ -130,7 +165,8 @@ int launch_extend(ExtendArgs& a, ExtendKv4Args* kv4, const void* fn, const int32
                   const int32_t* all_lens, void* workspace, size_t workspace_bytes, int32_t batch,
                   int64_t first, int32_t head_dim, int32_t dtype, void* hip_stream) {
   // without a workspace for the partials the keys are not split
-  a.split = extend_split(batch, new_lens, all_lens, a.hkv, a.group, a.window);
+  a.split = kv4 ? extend_split_kv4(batch, new_lens, all_lens, a.hkv, a.group, head_dim, a.window)
+                : extend_split(batch, new_lens, all_lens, a.hkv, a.group, a.window);
   if (a.split > 1) {
     size_t off_o, off_m, off_l, total;
     partials_layout_rows(first * (a.hkv * a.group) * a.split, head_dim, &off_o, &off_m, &off_l, &total);
@@ -192,22 +228,38 @@ int launch_extend(ExtendArgs& a, ExtendKv4Args* kv4, const void* fn, const int32
 }  // namespace
 }  // namespace dk
 
-extern "C" size_t dk_extend_workspace_bytes(int32_t batch, const int32_t* new_lens,
-                                            const int32_t* all_lens, int32_t num_q_heads,
-                                            int32_t num_kv_heads, int32_t head_dim,
-                                            int32_t window) {
+namespace {
+size_t extend_workspace(int32_t batch, const int32_t* new_lens, const int32_t* all_lens,
+                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t window,
+                        bool kv4) {
   using namespace dk;
   if (batch <= 0 || !new_lens || !all_lens || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_q_heads % num_kv_heads != 0 || head_dim <= 0 || window < 0)
     return 0;
-  const int s = extend_split(batch, new_lens, all_lens, num_kv_heads, num_q_heads / num_kv_heads,
-                             window);
+  const int32_t group = num_q_heads / num_kv_heads;
+  const int s = kv4 ? extend_split_kv4(batch, new_lens, all_lens, num_kv_heads, group, head_dim, window)
+                    : extend_split(batch, new_lens, all_lens, num_kv_heads, group, window);
   if (s == 1) return 0;
   int64_t tokens = 0;
   for (int32_t b = 0; b < batch; ++b) tokens += std::max(new_lens[b], 0);
   size_t o, m, l, total;
   partials_layout_rows(tokens * num_q_heads * s, head_dim, &o, &m, &l, &total);
   return total;
+}
+}  // namespace
+
+extern "C" size_t dk_extend_workspace_bytes(int32_t batch, const int32_t* new_lens,
+                                            const int32_t* all_lens, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim,
+                                            int32_t window) {
+  return extend_workspace(batch, new_lens, all_lens, num_q_heads, num_kv_heads, head_dim, window, false);
+}
+
+extern "C" size_t dk_extend_kv4_workspace_bytes(int32_t batch, const int32_t* new_lens,
+                                                const int32_t* all_lens, int32_t num_q_heads,
+                                                int32_t num_kv_heads, int32_t head_dim,
+                                                int32_t window) {
+  return extend_workspace(batch, new_lens, all_lens, num_q_heads, num_kv_heads, head_dim, window, true);
 }
 
 extern "C" int dk_extend_attention(

@@ -271,10 +271,10 @@ decltype(&dk_grow_block_tables) g_grow = nullptr;
 decltype(&dk_kv4_write) g_kv4_write = nullptr;
 decltype(&dk_kv4_read) g_kv4_read = nullptr;
 decltype(&dk_extend_attention_kv4) g_extend = nullptr;
-decltype(&dk_extend_workspace_bytes) g_extend_bytes = nullptr;
+decltype(&dk_extend_kv4_workspace_bytes) g_extend_bytes = nullptr;
 
-// bind_paging(grow_block_tables, kv4_write, kv4_read, extend_attention_kv4, extend_workspace_bytes:
-// addresses), after bind()
+// bind_paging(grow_block_tables, kv4_write, kv4_read, extend_attention_kv4,
+// extend_kv4_workspace_bytes: addresses), after bind()
 PyObject* bind_paging(PyObject*, PyObject* args) {
   unsigned long long grow, write, read, extend, bytes;
   if (!PyArg_ParseTuple(args, "KKKKK", &grow, &write, &read, &extend, &bytes)) return nullptr;

@@ -117,6 +117,8 @@ SIGNATURES = {
                                    _I64, _I32, _P]),
     "dk_extend_workspace_bytes": (_SZ, [_I32, ctypes.POINTER(_I32), ctypes.POINTER(_I32), _I32,
                                         _I32, _I32, _I32]),
+    "dk_extend_kv4_workspace_bytes": (_SZ, [_I32, ctypes.POINTER(_I32), ctypes.POINTER(_I32), _I32,
+                                            _I32, _I32, _I32]),
     "dk_extend_attention": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, ctypes.POINTER(_I32),
                                            ctypes.POINTER(_I32), ctypes.POINTER(_I32), _P, _P, _SZ,
                                            _I32, _I64, _I32, _I32, _I32, _I64, _I32, _I32,

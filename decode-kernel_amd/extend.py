@@ -198,7 +198,7 @@ def extend_attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     lib = dk_lib.load()
     hq = q.shape[1]
     s = dk_lib.DkExtendStrides(q.stride(0), q.stride(1), 0, 0, 0, 0, out.stride(0), out.stride(1))
-    size = lib.dk_extend_workspace_bytes(n, ints[1], ints[2], hq, hkv, d, win)
+    size = lib.dk_extend_kv4_workspace_bytes(n, ints[1], ints[2], hq, hkv, d, win)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     rc = paging._call(
         dev, lib.dk_extend_attention_kv4, q.data_ptr(), cache.data_ptr(), cache.stride(0),

@@ -133,7 +133,7 @@ def _native():
             lib = dk_lib.load()
             module.bind_paging(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 lib.dk_grow_block_tables, lib.dk_kv4_write, lib.dk_kv4_read,
-                lib.dk_extend_attention_kv4, lib.dk_extend_workspace_bytes)))
+                lib.dk_extend_attention_kv4, lib.dk_extend_kv4_workspace_bytes)))
             _NATIVE = module
         else:
             _NATIVE = False

@@ -404,6 +404,10 @@ typedef struct dk_extend_strides {
 size_t dk_extend_workspace_bytes(int32_t batch, const int32_t* new_lens, const int32_t* all_lens,
                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                  int32_t window);
+/* The same for dk_extend_attention_kv4. */
+size_t dk_extend_kv4_workspace_bytes(int32_t batch, const int32_t* new_lens,
+                                     const int32_t* all_lens, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, int32_t window);
 
 /* Extend (prefill) attention over a token pool: request b's new_lens[b] new tokens are the
  * last of its all_lens[b] tokens; new token i (position p = all_lens[b] - new_lens[b] + i)
@@ -434,7 +438,7 @@ int dk_extend_attention(const void* q, const void* k_pool, const void* v_pool,
 /* dk_extend_attention over a 4-bit cache (DK_KV_MXFP4; kv_p, kv_h in bytes): the K and V of request
  * b's position p lie in page block_table[rows[b]][p / 16] (rows table_stride entries apart, num_rows
  * of them, max_blocks entries each; a page id outside [0, num_pages) gives NaN to the tokens that
- * attend to it). strides: q_b, q_h, o_b, o_h. The same workspace (dk_extend_workspace_bytes). In fp16,
+ * attend to it). strides: q_b, q_h, o_b, o_h. A workspace as there (dk_extend_kv4_workspace_bytes). In fp16,
  * cache values beyond twice fp16's range become infinite. No counterpart in the reference. */
 int dk_extend_attention_kv4(const void* q, const void* cache, int64_t kv_p, int64_t kv_h,
                             const int32_t* block_table, int64_t table_stride, int64_t num_rows,

@@ -70,6 +70,25 @@ def test_abi_refusals(kw, code):
         0, None, None) == code
 
 
+def test_workspace_bytes():
+    """Room for the partials of the split that a call takes: none for a short or an empty one, none past
+    what the tiles of a full chip take, never more than the largest split's."""
+    lib = dk_lib.load()
+
+    def need(new, alls, hq, hkv, d, window=0):
+        ints = ctypes.c_int32 * len(new)
+        return lib.dk_extend_kv4_workspace_bytes(len(new), ints(*new), ints(*alls), hq, hkv, d, window)
+
+    assert need([0, 0], [5, 0], 8, 2, 64) == need([3], [200], 8, 2, 64) == need([512], [512], 32, 8, 128) == 0
+    assert need([2048], [8192], 32, 8, 128) == 0 and need([-1], [5], 8, 2, 64) == 0
+    assert need([4], [8000], 8, 2, 64, window=100) == 0
+    for d in (64, 128, 256):
+        some = need([16], [8000], 32, 8, d)
+        ints = ctypes.c_int32 * 1
+        assert 0 < some <= lib.dk_extend_workspace_bytes(1, ints(16), ints(8000), 32, 8, d, 0)
+        assert some % (16 * 32 * (d + 2) * 4) == 0            # whole rows of O, m and l
+
+
 def _case(reqs, hq, hkv, d, dtype, seed):
     """reqs: (prefix, new) per request. Pages in random order, unused table entries outside the cache."""
     r = np.random.default_rng(seed)
@@ -260,7 +279,7 @@ def test_split_keys_keep_nan(d):
     q, cache, raw, table, rows, new, alls = _case([(2990, 3)], 4, 2, d, torch.bfloat16, d)
     t = torch.from_numpy(table).to(DEV)
     i32 = ctypes.c_int32 * 1
-    assert dk_lib.load().dk_extend_workspace_bytes(1, i32(3), i32(2993), 4, 2, d, 0) > 0
+    assert dk_lib.load().dk_extend_kv4_workspace_bytes(1, i32(3), i32(2993), 4, 2, d, 0) > 0
     want = extend.extend_attention_kv4(q, cache, t, rows, new, alls)
     tb = table.copy()
     tb[rows[0], 187] = 2 ** 31 - 1                           # tokens 2992 ..: the last query's alone
