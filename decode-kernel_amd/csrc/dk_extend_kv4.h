@@ -450,8 +450,6 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
   __syncthreads();
   for (int j = kbeg; j < kend; ++j) {
     const int buf = (j - kbeg) & 1 ? BUF : 0;
-    load_tile();                      // after the last tile a page of the request again, for nobody
-    load_id(j + 2);
     auto fix = [&] {
       if ((j + 2) * BN > rq.n_all || bad || any_nan()) fix_tile(j + 1, BUF - buf);
     };
@@ -474,6 +472,8 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
       if constexpr (NB == 2) read_ks(1, buf, ks1);
 #pragma unroll
       for (int g = 0; g < kAhead; ++g) fetch(g);
+      load_tile();                    // after the last tile a page of the request again, for nobody
+      load_id(j + 2);
       for_each<NB * KM>([&](auto g) {
         constexpr int n = g.value / KM, m = g.value % KM;
         f32x16& x = n ? s1 : s0;
@@ -519,6 +519,8 @@ __global__ __launch_bounds__(kExtendThreads, (kv4_extend_resident(D, CAP))) void
         pin();
       });
     } else {
+      load_tile();
+      load_id(j + 2);
       fix();
       store_tile(BUF - buf);
     }
